@@ -104,7 +104,7 @@ def workspace(case):
     api.lib.qw4cu_set_stream(torch.cuda.current_stream().cuda_stream or 1)          # 1: the legacy default stream by its handle
     if case["op"].startswith("adapter"):
         return tuning.TuneWork(api, tokens=case["tokens"], slots=case["slots"], rank=case["rank"])
-    return tuning.TuneWork(api, tokens=case["tokens"], experts=case["experts"], top_k=case["top_k"])
+    return tuning.TuneWork(api, tokens=case["tokens"], experts=case["experts"])
 
 
 def prepare(case, seed):
@@ -149,6 +149,8 @@ def prepare(case, seed):
         s.work = workspace(case)
         if case["op"].startswith("adapter"):
             s.adapters = s.work.adapters(s.a.data_ptr(), s.b.data_ptr(), s.scale.data_ptr(), GGUF[case["dtype"]], slots, r, k, n)
+        else:
+            s.config = s.work.router(e, top, case["norm"])
     return s
 
 
@@ -233,11 +235,11 @@ def run(s):
         s.work.adapter_backward(s.adapters, s.x.data_ptr(), s.slot.data_ptr(), s.dy.data_ptr(), s.base.data_ptr(), o["dx"].data_ptr(),
                                 o["da"].data_ptr(), o["db"].data_ptr(), c["tokens"])
     elif c["op"] == "balance forward":
-        s.work.balance_forward(s.logits.data_ptr(), s.ids.data_ptr(), s.mask.data_ptr() if s.mask is not None else None, c["tokens"],
+        s.work.balance_forward(s.config, s.logits.data_ptr(), s.ids.data_ptr(), s.mask.data_ptr() if s.mask is not None else None, c["tokens"],
                                o["counts"].data_ptr(), o["prob_sums"].data_ptr(), o["loss"].data_ptr())
     else:
-        s.work.balance_backward(s.logits.data_ptr(), s.ids.data_ptr(), s.mask.data_ptr() if s.mask is not None else None, c["tokens"],
-                                s.counts.data_ptr(), s.loss_grad, s.weights_grad.data_ptr(), o["grad"].data_ptr(), c["norm"])
+        s.work.balance_backward(s.config, s.logits.data_ptr(), s.ids.data_ptr(), s.mask.data_ptr() if s.mask is not None else None, c["tokens"],
+                                s.counts.data_ptr(), s.loss_grad, s.weights_grad.data_ptr(), o["grad"].data_ptr())
     return o
 
 
