@@ -532,6 +532,89 @@ Qwen4Status qw4cu_verify_keep(QW4CuVerify *verify, size_t keep, Qwen4Error *err)
 uint64_t qw4cu_verify_position(const QW4CuVerify *verify);
 size_t qw4cu_verify_pending(const QW4CuVerify *verify);
 
+/* ------------------------------------------------------------------------------------
+ * A layer that is adapted and trained: low-rank adapters of many requests beside a projection they
+ * share, and the balance loss of a router, each with its gradients (csrc/adapters.cu, csrc/balance.cu).
+ * No counterpart in the reference, whose weights are frozen.
+ *
+ * All data pointers are device pointers, values FP32 unless said otherwise, last axis contiguous; a
+ * float's alignment is enough everywhere (rows on 16-byte boundaries are read with wider loads).  The
+ * calls enqueue on the stream in force (qw4cu_set_stream) and return without waiting, allocate nothing
+ * and may be captured into a CUDA graph.  What the kernels find (an id out of range, a logit row
+ * without a softmax) is reported by qw4cu_tune_work_sync and latches the workspace until
+ * qw4cu_tune_work_reset.  Calls on one workspace must follow one another on the GPU (one stream, or
+ * streams that wait for each other; graphs captured with it likewise); calls that may overlap need a
+ * workspace each.  A workspace belongs to the device that was current when it was made.  Results
+ * do not depend on timing: every sum has a fixed order.
+ * ---------------------------------------------------------------------------------- */
+typedef struct QW4CuTuneWork QW4CuTuneWork;
+
+/* What the calls on a workspace may ask for.  slots = 0: no adapters; experts = 0: no balance loss. */
+typedef struct {
+    size_t tokens;                         /* 1 .. QW4CU_TUNE_MAX_TOKENS */
+    uint32_t slots, rank;                  /* adapters: up to 1024 slots, rank 1 .. 128 */
+    uint32_t experts;                      /* balance loss: up to 4096 experts */
+} QW4CuTuneLimits;
+#define QW4CU_TUNE_MAX_TOKENS (1u << 20)
+#define QW4CU_TUNE_MAX_SLOTS 1024u
+#define QW4CU_TUNE_MAX_RANK 128u
+#define QW4CU_TUNE_MAX_EXPERTS 4096u
+
+Qwen4Status qw4cu_tune_work_create(const QW4CuTuneLimits *limits, QW4CuTuneWork **out, Qwen4Error *err);
+void qw4cu_tune_work_destroy(QW4CuTuneWork *work);
+size_t qw4cu_tune_work_device_bytes(const QW4CuTuneWork *work);
+/* Waits for the stream in force and turns what the kernels found into a status: QW4_RANGE (a slot or expert id
+ * out of range), QW4_NONFINITE (a row of logits that has no softmax; err->row is the lowest). */
+Qwen4Status qw4cu_tune_work_sync(QW4CuTuneWork *work, Qwen4Error *err);
+Qwen4Status qw4cu_tune_work_reset(QW4CuTuneWork *work, Qwen4Error *err);
+
+/* Adapters beside one projection of k inputs and n outputs: slot s holds A_s [rank, k] and B_s [n, rank], and adds
+ * scale_s B_s (A_s x) to what the projection gives.  An adapter of lower rank is padded with zero rows of A and
+ * zero columns of B.  type: 0 F32, 1 F16, 30 BF16 (GGUF tensor ids), for both. */
+typedef struct {
+    const void *a;                         /* [slots, rank, k] */
+    const void *b;                         /* [slots, n, rank] */
+    const float *scale;                    /* [slots]; NULL: 1 */
+    uint32_t type, slots, rank;
+    size_t k, n;
+} QW4CuAdapters;
+#define QW4CU_NO_ADAPTER 0xffffffffu
+
+/* y[t] = base[t] + scale_s B_s (A_s x[t]) with s = slots_dev[t]; y[t] = base[t] where that is QW4CU_NO_ADAPTER (or
+ * out of range).  base NULL: zero; base may be y itself (same pitch), otherwise y must not overlap what is read.
+ * Pitches are bytes between rows.  x [tokens, k], base and y [tokens, n].  Tokens of a slot may lie anywhere in the
+ * batch.  Products of F16 and BF16 adapters are exact and summed in FP32; x, and F32 adapters, enter the tensor
+ * cores as a sum of three bf16 values (24 bits). */
+Qwen4Status qw4cu_adapter_forward_device(const QW4CuAdapters *adapters, const float *x_dev, size_t x_pitch, const uint32_t *slots_dev,
+                                         const float *base_dev, size_t base_pitch, float *y_dev, size_t y_pitch, size_t tokens,
+                                         QW4CuTuneWork *work, Qwen4Error *err);
+/* Its gradients, for dy [tokens, n]:  g[t] = scale_s B_s^T dy[t];  dx[t] = base[t] + A_s^T g[t] (base: the gradient that came
+ * through the projection itself; as above);  da [slots, rank, k] = sum over the slot's tokens of g x^T;  db [slots, n, rank] =
+ * scale_s times the sum of dy (A_s x)^T.  da and db are dense FP32 and overwritten, zero for slots without tokens.
+ * dx_dev may be NULL, and da_dev and db_dev too (together). */
+Qwen4Status qw4cu_adapter_backward_device(const QW4CuAdapters *adapters, const float *x_dev, size_t x_pitch, const uint32_t *slots_dev,
+                                          const float *dy_dev, size_t dy_pitch, const float *base_dev, size_t base_pitch, float *dx_dev,
+                                          size_t dx_pitch, float *da_dev, float *db_dev, size_t tokens, QW4CuTuneWork *work, Qwen4Error *err);
+
+/* Balance loss of a router over one batch.  With p[t] = softmax(logits[t]) for the N tokens that mask_dev (uint8 [tokens], nonzero
+ * = counts; NULL: all) leaves:
+ *     counts[e]    = number of (token, slot) pairs of those tokens with ids[t, slot] = e      uint32 [experts + 1], counts[experts] = N
+ *     prob_sums[e] = sum of p[t, e] over those tokens                                         [experts]
+ *     loss         = experts / N^2 * sum over e of counts[e] * prob_sums[e]                   [1]; 0 when N = 0
+ * logits [tokens, experts] with logits_pitch bytes between rows; ids [tokens, top_k] dense, distinct within a token.  A logit of -inf
+ * is an expert left out (p = 0); a row with a NaN, a +inf or nothing but -inf has no softmax: loss and prob_sums are
+ * then NaN.  Rows that the mask leaves out are not read.  Of config, experts, top_k and norm_topk_prob are used. */
+Qwen4Status qw4cu_balance_forward_device(const Qwen4MoeConfig *config, const float *logits_dev, size_t logits_pitch, const uint32_t *ids_dev,
+                                         const uint8_t *mask_dev, size_t tokens, uint32_t *counts_dev, float *prob_sums_dev, float *loss_dev,
+                                         QW4CuTuneWork *work, Qwen4Error *err);
+/* Gradient of the router's logits: of loss_grad * loss, with the counts as they are (they may have been summed over
+ * ranks, N included, for a loss over the whole batch of a job), plus, where weights_grad_dev [tokens, top_k] is given, that of the
+ * route weights (normalised over the chosen experts if config->norm_topk_prob, plain probabilities otherwise) for it.
+ * grad [tokens, experts] is overwritten; rows that the mask leaves out are zero. */
+Qwen4Status qw4cu_balance_backward_device(const Qwen4MoeConfig *config, const float *logits_dev, size_t logits_pitch, const uint32_t *ids_dev,
+                                          const uint8_t *mask_dev, size_t tokens, const uint32_t *counts_dev, float loss_grad,
+                                          const float *weights_grad_dev, float *grad_dev, size_t grad_pitch, QW4CuTuneWork *work, Qwen4Error *err);
+
 /* Raw device memory and transfers for callers that keep activations in HBM. */
 void *qw4cu_malloc(size_t bytes);
 void qw4cu_free(void *device_pointer);

@@ -85,6 +85,15 @@ class QW4CuGgufSlice(C.Structure):
                 ("data_offset", C.c_uint64), ("file_bytes", C.c_uint64)]
 
 
+class QW4CuTuneLimits(C.Structure):
+    _fields_ = [("tokens", C.c_size_t), ("slots", C.c_uint32), ("rank", C.c_uint32), ("experts", C.c_uint32)]
+
+
+class QW4CuAdapters(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("type", C.c_uint32), ("slots", C.c_uint32),
+                ("rank", C.c_uint32), ("k", C.c_size_t), ("n", C.c_size_t)]
+
+
 class Qwen4MoeWeights(C.Structure):
     _fields_ = [(name, QW4PackedCpuView) for name in
                 ("router", "gate", "up", "down", "shared_gate", "shared_up", "shared_down",
@@ -264,6 +273,15 @@ class MoeApi:
             "qw4cu_gguf_slice_describe": ([C.c_char_p, C.c_uint32, C.POINTER(QW4CuGgufSlice), C.POINTER(Qwen4Error)], C.c_int),
             "qw4cu_moe_create_from_gguf": ([C.c_char_p, C.c_uint32, C.POINTER(P), C.POINTER(QW4CuGgufSlice), C.POINTER(Qwen4Error)], C.c_int),
             "qw4cu_device_synchronize": ([], C.c_int),
+            "qw4cu_tune_work_create": ([C.POINTER(QW4CuTuneLimits), C.POINTER(P), E], C.c_int),
+            "qw4cu_tune_work_destroy": ([P], None),
+            "qw4cu_tune_work_device_bytes": ([P], C.c_size_t),
+            "qw4cu_tune_work_sync": ([P, E], C.c_int),
+            "qw4cu_tune_work_reset": ([P, E], C.c_int),
+            "qw4cu_adapter_forward_device": ([P, P, C.c_size_t, P, P, C.c_size_t, P, C.c_size_t, C.c_size_t, P, P], C.c_int),
+            "qw4cu_adapter_backward_device": ([P, P, C.c_size_t, P, P, C.c_size_t, P, C.c_size_t, P, C.c_size_t, P, P, C.c_size_t, P, P], C.c_int),
+            "qw4cu_balance_forward_device": ([P, P, C.c_size_t, P, P, C.c_size_t, P, P, P, P, P], C.c_int),
+            "qw4cu_balance_backward_device": ([P, P, C.c_size_t, P, P, C.c_size_t, P, C.c_float, P, P, C.c_size_t, P, P], C.c_int),
         }
         for name, (argtypes, restype) in sig.items():
             fn = getattr(lib, name)

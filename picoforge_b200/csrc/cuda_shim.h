@@ -239,6 +239,26 @@ int qw4sh_expert_tc(int mode, int prefill, const QW4ShTensor *w0, const QW4ShTen
 int qw4sh_observed_forward(const QW4ShLayer *layer, const QW4ShWork *work, const float *x, float *y, size_t tokens, const float *x_host,
                            size_t x_host_pitch, size_t token0, QW4MoeObserver observer, void *ctx);
 int qw4sh_route_forward(const QW4ShLayer *layer, const QW4ShWork *work, const float *x, size_t tokens, int router_mode);
+/* Adapters and balance loss (adapters.cu, balance.cu): device scratch of one QW4CuTuneWork. */
+typedef struct {
+    uint32_t *status;             /* [4]: error bits, lowest bad row */
+    /* balance loss: sums over the CTAs of a launch, zero between launches */
+    unsigned long long *prob_sums;    /* [experts] units of 2^-40 */
+    uint32_t *counts;             /* [experts + 1], and one ticket behind them */
+    /* adapters: A x and B^T dy of every token */
+    float *h, *g;                 /* [tokens, rank] */
+} QW4ShTune;
+int qw4sh_balance_forward(const QW4ShTune *tune, uint32_t experts, uint32_t k, const float *logits, size_t pitch, const uint32_t *ids,
+                          const uint8_t *mask, size_t tokens, uint32_t *counts, float *prob_sums, float *loss, void *stream);
+int qw4sh_balance_backward(const QW4ShTune *tune, uint32_t experts, uint32_t k, int norm, const float *logits, size_t pitch, const uint32_t *ids,
+                           const uint8_t *mask, size_t tokens, const uint32_t *counts, float loss_grad, const float *weights_grad, float *grad,
+                           size_t grad_pitch, void *stream);
+int qw4sh_adapter_forward(const QW4ShTune *tune, const QW4CuAdapters *ad, const float *x, size_t x_pitch, const uint32_t *slots,
+                          const float *base, size_t base_pitch, float *y, size_t y_pitch, size_t tokens, void *stream);
+int qw4sh_adapter_backward(const QW4ShTune *tune, const QW4CuAdapters *ad, const float *x, size_t x_pitch, const uint32_t *slots,
+                           const float *dy, size_t dy_pitch, const float *base, size_t base_pitch, float *dx, size_t dx_pitch,
+                           float *da, float *db, size_t tokens, void *stream);
+
 /* Caller-provided stream (NULL: back to the library's own).  current_stream returns the one in force. */
 int qw4sh_set_stream(void *stream);
 int qw4sh_current_stream(void **stream);
