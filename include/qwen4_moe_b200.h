@@ -568,7 +568,7 @@ size_t qw4cu_tune_work_device_bytes(const QW4CuTuneWork *work);
 Qwen4Status qw4cu_tune_work_sync(QW4CuTuneWork *work, Qwen4Error *err);
 Qwen4Status qw4cu_tune_work_reset(QW4CuTuneWork *work, Qwen4Error *err);
 
-/* Adapters beside one projection of k inputs and n outputs: slot s holds A_s [rank, k] and B_s [n, rank], and adds
+/* Adapters beside one projection of k inputs and n outputs (up to 2^20 each): slot s holds A_s [rank, k] and B_s [n, rank], and adds
  * scale_s B_s (A_s x) to what the projection gives.  An adapter of lower rank is padded with zero rows of A and
  * zero columns of B.  type: 0 F32, 1 F16, 30 BF16 (GGUF tensor ids), for both. */
 typedef struct {

@@ -245,9 +245,15 @@ typedef struct {
     /* balance loss: sums over the CTAs of a launch, zero between launches */
     unsigned long long *prob_sums;    /* [experts] units of 2^-40 */
     uint32_t *counts;             /* [experts + 1], and one ticket behind them */
-    /* adapters: A x and B^T dy of every token */
-    float *h, *g;                 /* [tokens, rank] */
+    /* adapters: tokens sorted by slot, and tiles of them (16 bytes each) */
+    uint32_t *order, *offsets;    /* [tokens], [slots + 2] */
+    void *tiles;                  /* [qw4sh_adapter_tiles(tokens, slots)] */
+    uint32_t *n_tiles;
+    /* A x and B^T dy of every token, in that order, cut in three bf16 values */
+    void *h, *g;                  /* [3][tokens][qw4sh_adapter_rank(rank)] */
 } QW4ShTune;
+size_t qw4sh_adapter_tiles(size_t tokens, uint32_t slots);
+uint32_t qw4sh_adapter_rank(uint32_t rank);
 int qw4sh_balance_forward(const QW4ShTune *tune, uint32_t experts, uint32_t k, const float *logits, size_t pitch, const uint32_t *ids,
                           const uint8_t *mask, size_t tokens, uint32_t *counts, float *prob_sums, float *loss, void *stream);
 int qw4sh_balance_backward(const QW4ShTune *tune, uint32_t experts, uint32_t k, int norm, const float *logits, size_t pitch, const uint32_t *ids,

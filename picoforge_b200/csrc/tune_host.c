@@ -60,7 +60,10 @@ Qwen4Status qw4cu_tune_work_create(const QW4CuTuneLimits *limits, QW4CuTuneWork 
     w->device = qw4sh_current_device();
     size_t at = 0;
     const size_t status = take(&at, 16), sums = take(&at, (size_t)l.experts * 8), counts = take(&at, ((size_t)l.experts + 2) * 4);
-    const size_t rows = l.slots ? l.tokens * l.rank * 4 : 0, h = take(&at, rows), g = take(&at, rows);
+    const bool adapters = l.slots != 0;
+    const size_t order = take(&at, adapters ? l.tokens * 4 : 0), offsets = take(&at, adapters ? ((size_t)l.slots + 2) * 4 : 0);
+    const size_t tiles = take(&at, adapters ? qw4sh_adapter_tiles(l.tokens, l.slots) * 16 : 0), n_tiles = take(&at, 4);
+    const size_t rows = adapters ? 3 * l.tokens * qw4sh_adapter_rank(l.rank) * 2 : 0, h = take(&at, rows), g = take(&at, rows);
     w->device_bytes = at;
     w->block = qw4sh_malloc(at);
     void *stream = NULL;
@@ -74,8 +77,12 @@ Qwen4Status qw4cu_tune_work_create(const QW4CuTuneLimits *limits, QW4CuTuneWork 
     w->d.status = (uint32_t *)(w->block + status);
     w->d.prob_sums = (unsigned long long *)(w->block + sums);
     w->d.counts = (uint32_t *)(w->block + counts);
-    w->d.h = (float *)(w->block + h);
-    w->d.g = (float *)(w->block + g);
+    w->d.order = (uint32_t *)(w->block + order);
+    w->d.offsets = (uint32_t *)(w->block + offsets);
+    w->d.tiles = w->block + tiles;
+    w->d.n_tiles = (uint32_t *)(w->block + n_tiles);
+    w->d.h = w->block + h;
+    w->d.g = w->block + g;
     if (qw4sh_memset_async(w->block, 0, at, stream) || status_clear(w, stream) || qw4sh_stream_sync(stream)) {
         const Qwen4Status st = cuda_answer(err, "workspace clear");
         qw4cu_tune_work_destroy(w);
@@ -108,6 +115,7 @@ Qwen4Status qw4cu_tune_work_sync(QW4CuTuneWork *w, Qwen4Error *err) {
     const uint32_t bits = w->status_host[0], row = w->status_host[1];
     if (!bits) return answer(err, QW4_OK, "");
     w->failed = true;
+    if (bits & QW4SH_ERR_STATE) return answer(err, QW4_GPU_ERROR, "device state error");
     if (bits & QW4SH_ERR_BOUNDS) return answer(err, QW4_RANGE, "adapter slot or expert id out of range");
     const Qwen4Status bad = answer(err, QW4_NONFINITE, "a row of logits has no softmax");
     if (err && row != UINT32_MAX) err->row = row;
@@ -162,10 +170,10 @@ static Qwen4Status apart(const Bytes *written, size_t nw, const Bytes *read, siz
     return QW4_OK;
 }
 
-enum { MAX_DIM = 1u << 24 };
+enum { MAX_DIM = 1u << 20 };
 static Qwen4Status check_adapters(const QW4CuAdapters *ad, const QW4CuTuneWork *w, Bytes *a, Bytes *b, Bytes *scale, Qwen4Error *err) {
     if (!ad) return answer(err, QW4_INVALID_ARGUMENT, "null adapters");
-    if (!ad->k || !ad->n || ad->k > MAX_DIM || ad->n > MAX_DIM) return answer(err, QW4_SHAPE, "projection dimensions outside 1 .. 2^24");
+    if (!ad->k || !ad->n || ad->k > MAX_DIM || ad->n > MAX_DIM) return answer(err, QW4_SHAPE, "projection dimensions outside 1 .. 2^20");
     if (!ad->slots || !ad->rank) return answer(err, QW4_SHAPE, "adapters of no slot or rank zero");
     if (ad->slots > w->limits.slots || ad->rank > w->limits.rank) return answer(err, QW4_CAPACITY, "adapter slots or rank beyond the workspace's");
     if (ad->type != 0 && ad->type != 1 && ad->type != 30) return answer(err, QW4_TYPE, "adapters are F32, F16 or BF16");
