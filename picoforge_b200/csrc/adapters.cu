@@ -31,7 +31,7 @@ namespace {
 
 constexpr uint32_t THREADS = 256, TM = 128;                  // tokens per tile: tcgen05's M (shrink) or most N (expand)
 constexpr uint32_t KC = 64;                                  // shrink: columns per step
-constexpr uint32_t TC = 32;                                  // outer: tokens per step
+constexpr uint32_t TC = 64;                                  // outer: tokens per step
 
 // ---- PTX ------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -121,31 +121,35 @@ template <int PLANES> __device__ __forceinline__ void put_cut(uint32_t addr, uin
     }
 }
 
-// Four neighbouring values of a row as they are in memory; `valid` of them exist.  `wide`: rows start on a boundary of four values.
+// Four neighbouring values of a row as they are in memory.  Loads have no condition (a branch around one makes its result wait at the
+// join, and the loads of a step then follow one another): places that do not exist are read at the last one that does, and zeroed
+// (`keep`) when they are cut.
 template <typename W> struct Four;
 template <> struct Four<float> {
     static constexpr int PLANES = 3;
     float4 v;
-    __device__ __forceinline__ void load(const float *p, int valid, bool wide) {
-        if (valid >= 4 && wide) { v = *(const float4 *)p; return; }
-        v = make_float4(0, 0, 0, 0);
-        if (valid > 0) v.x = p[0];
-        if (valid > 1) v.y = p[1];
-        if (valid > 2) v.z = p[2];
-        if (valid > 3) v.w = p[3];
+    __device__ __forceinline__ void load4(const float *p) { v = *(const float4 *)p; }
+    __device__ __forceinline__ void load1(const float *row, uint32_t c, uint32_t last) {
+        v = make_float4(row[min(c, last)], row[min(c + 1, last)], row[min(c + 2, last)], row[min(c + 3, last)]);
+    }
+    __device__ __forceinline__ void keep(int valid) {
+        if (valid < 1) v.x = 0;
+        if (valid < 2) v.y = 0;
+        if (valid < 3) v.z = 0;
+        if (valid < 4) v.w = 0;
     }
     __device__ __forceinline__ void put(uint32_t addr, uint32_t step) const { put_cut<3>(addr, step, v); }
 };
 template <typename H> struct Four16 {
     uint2 v;
-    __device__ __forceinline__ void load(const H *q, int valid, bool wide) {
-        const uint16_t *p = (const uint16_t *)q;
-        if (valid >= 4 && wide) { v = *(const uint2 *)p; return; }
-        v = make_uint2(0, 0);
-        if (valid > 0) v.x = p[0];
-        if (valid > 1) v.x |= (uint32_t)p[1] << 16;
-        if (valid > 2) v.y = p[2];
-        if (valid > 3) v.y |= (uint32_t)p[3] << 16;
+    __device__ __forceinline__ void load4(const H *p) { v = *(const uint2 *)p; }
+    __device__ __forceinline__ void load1(const H *q, uint32_t c, uint32_t last) {
+        const uint16_t *row = (const uint16_t *)q;
+        v = make_uint2(row[min(c, last)] | (uint32_t)row[min(c + 1, last)] << 16, row[min(c + 2, last)] | (uint32_t)row[min(c + 3, last)] << 16);
+    }
+    __device__ __forceinline__ void keep(int valid) {
+        v.x &= valid < 1 ? 0u : valid < 2 ? 0xffffu : 0xffffffffu;
+        v.y &= valid < 3 ? 0u : valid < 4 ? 0xffffu : 0xffffffffu;
     }
 };
 template <> struct Four<__nv_bfloat16> : Four16<__nv_bfloat16> {
@@ -159,9 +163,72 @@ template <> struct Four<__half> : Four16<__half> {
         put_cut<2>(addr, step, make_float4(a.x, a.y, b.x, b.y));
     }
 };
+// How many of four places from c on lie before `end`.
+__device__ __forceinline__ int places(uint32_t c, uint32_t end) { return c < end ? (int)min(4u, end - c) : 0; }
 
-// The adapters of all slots as [rank, width] matrices: WIDE: rows of the rank axis (A), else rows of the wide axis (B).
-template <typename W> struct Mat { const W *p; uint64_t slot; uint32_t rank; uint64_t width; bool wide; };
+// The adapters of all slots as [rank, width] matrices: wide: rows of the rank axis (A), else rows of the wide axis (B).  `fours`: rows
+// start on a boundary of four values and end on one.
+template <typename W> struct Mat { const W *p; uint64_t slot; uint32_t rank, width; bool wide, fours; };
+
+// A run of LEN columns of a slot's matrix (rank padded to RP) on its way into the operand tiles Wide (RP x LEN) or Tall (LEN x RP).
+// Where runs of four lie on their boundaries a thread keeps the places it reads in such runs and moves them on from run to run.
+template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
+    static constexpr uint32_t UNITS = RP * LEN / 4 / THREADS, PLANES = Four<W>::PLANES;
+    using Wide = Tile<RP, LEN, PLANES>;
+    using Tall = Tile<LEN, RP, PLANES>;
+    static constexpr uint32_t BYTES = Wide::BYTES > Tall::BYTES ? Wide::BYTES : Tall::BYTES;
+    Four<W> v[UNITS];
+    uint32_t at[UNITS];
+    static __device__ __forceinline__ uint32_t wide_r(uint32_t i) { return (threadIdx.x + i * THREADS) / (LEN / 4); }
+    static __device__ __forceinline__ uint32_t wide_c(uint32_t i) { return (threadIdx.x + i * THREADS) % (LEN / 4) * 4; }
+    static __device__ __forceinline__ uint32_t tall_c(uint32_t i) { return (threadIdx.x + i * THREADS) / (RP / 4); }
+    static __device__ __forceinline__ uint32_t tall_r(uint32_t i) { return (threadIdx.x + i * THREADS) % (RP / 4) * 4; }
+    __device__ __forceinline__ void begin(const Mat<W> &m, uint32_t c0) {
+#pragma unroll
+        for (uint32_t i = 0; i < UNITS; i++)
+            at[i] = m.wide ? (min(wide_r(i), m.rank - 1) * m.width + c0 + wide_c(i)) / 4 : ((c0 + tall_c(i)) * m.rank + min(tall_r(i), (m.rank - 1) & ~3u)) / 4;
+    }
+    // columns c0 .. c0 + LEN of w, which end at `end`
+    __device__ __forceinline__ void load(const Mat<W> &m, const W *w, uint32_t c0, uint32_t end) {
+        if (m.fours && c0 + LEN <= end) {
+            const uint32_t step = m.wide ? LEN / 4 : LEN / 4 * m.rank;
+#pragma unroll
+            for (uint32_t i = 0; i < UNITS; i++) { v[i].load4(w + (uint64_t)at[i] * 4); at[i] += step; }
+        } else if (m.wide) {
+#pragma unroll 1
+            for (uint32_t i = 0; i < UNITS; i++) {
+                Four<W> f;
+                f.load1(w + (uint64_t)min(wide_r(i), m.rank - 1) * m.width, c0 + wide_c(i), end - 1);
+                set(i, f);
+            }
+        } else {
+#pragma unroll 1
+            for (uint32_t i = 0; i < UNITS; i++) {
+                Four<W> f;
+                f.load1(w + (uint64_t)min(c0 + tall_c(i), end - 1) * m.rank, tall_r(i), m.rank - 1);
+                set(i, f);
+            }
+        }
+    }
+    __device__ __forceinline__ void set(uint32_t i, const Four<W> &f) {
+#pragma unroll
+        for (uint32_t j = 0; j < UNITS; j++) if (i == j) v[j] = f;
+    }
+    __device__ __forceinline__ void put(const Mat<W> &m, uint32_t c0, uint32_t end, uint32_t addr) {
+        if (m.rank != RP || c0 + LEN > end)
+#pragma unroll
+            for (uint32_t i = 0; i < UNITS; i++) {
+                if (m.wide) v[i].keep(wide_r(i) < m.rank ? places(c0 + wide_c(i), end) : 0);
+                else v[i].keep(c0 + tall_c(i) < end ? places(tall_r(i), m.rank) : 0);
+            }
+        if (m.wide)
+#pragma unroll
+            for (uint32_t i = 0; i < UNITS; i++) v[i].put(addr + Wide::at(wide_r(i), wide_c(i)), Wide::PLANE);
+        else
+#pragma unroll
+            for (uint32_t i = 0; i < UNITS; i++) v[i].put(addr + Tall::at(tall_c(i), tall_r(i)), Tall::PLANE);
+    }
+};
 
 // ---- lists ------------------------------------------------------------------------------------------------------------------
 // Tokens sorted by slot (tokens without one last, in the group `slots`), in the order of the batch inside a slot; tiles of up to
@@ -171,33 +238,49 @@ struct ATile { uint32_t slot, first, rows, pad; };
 __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__restrict__ ids, uint32_t T, uint32_t S, uint32_t *__restrict__ order,
                                                              uint32_t *__restrict__ offsets, ATile *__restrict__ tiles, uint32_t *__restrict__ n_tiles,
                                                              uint32_t *status) {
-    extern __shared__ uint32_t counts[];                     // [warps][S + 1]
+    extern __shared__ uint32_t counts[];                     // [warps][S + 1], then the groups' tokens [S + 1]
     __shared__ uint32_t sums[2][32];
     const uint32_t G = S + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t per = ((T + 31) / 32 + 31) & ~31u, first = warp * per, end = min(T, first + per);
+    const uint32_t per = ((T + 31) / 32 + 31) & ~31u, first = min(T, warp * per), end = min(T, first + per);
+    uint32_t *mine = counts + warp * G, *totals = counts + 32 * G;
+    grid_go();                                               // the tiles' CTAs may take their places
+    constexpr uint32_t AHEAD = 8;                            // loads in flight
+    uint32_t s[AHEAD];
+    auto fetch = [&](uint32_t t0) {
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; i++) s[i] = ids[min(t0 + 32 * i + lane, T - 1)];
+    };
+    fetch(first);
     for (uint32_t i = threadIdx.x; i < 32 * G; i += 1024) counts[i] = 0;
     __syncthreads();
-    uint32_t *mine = counts + warp * G;
-    for (uint32_t t = first + lane; t - lane < end; t += 32) {
-        uint32_t s = 0xffffffffu;
-        if (t < end) {
-            s = ids[t];
-            if (s >= S) {
-                if (s != QW4CU_NO_ADAPTER) atomicOr(status, QW4SH_ERR_BOUNDS);
-                s = S;
-            }
+    for (uint32_t t0 = first; t0 < end; t0 += 32 * AHEAD) {
+        if (t0 != first) fetch(t0);
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; i++) {
+            if (t0 + 32 * i >= end) break;
+            const bool there = t0 + 32 * i + lane < end;
+            if (there && s[i] >= S && s[i] != QW4CU_NO_ADAPTER) atomicOr(status, QW4SH_ERR_BOUNDS);
+            const uint32_t g = there ? min(s[i], S) : 0xffffffffu, same = __match_any_sync(0xffffffffu, g);
+            if (there && __ffs(same) - 1 == (int)lane) mine[g] += __popc(same);
+            __syncwarp();
         }
-        const uint32_t same = __match_any_sync(0xffffffffu, s);
-        if (t < end && __ffs(same) - 1 == (int)lane) mine[s] += __popc(same);
-        __syncwarp();
     }
     __syncthreads();
-    // a thread per group (two where there are more than 1024): where the group and its tiles start
-    uint32_t total[2] = {0, 0}, rows_before = 0, tiles_before = 0;
-    for (uint32_t j = 0; j < 2; j++) {
-        const uint32_t g = 2 * threadIdx.x + j;
-        if (g < G) for (uint32_t w = 0; w < 32; w++) { const uint32_t c = counts[w * G + g]; counts[w * G + g] = total[j]; total[j] += c; }
+    // where each warp's run of a group starts inside it: a warp per group, a lane per run
+    for (uint32_t g = warp; g < G; g += 32) {
+        const uint32_t c = counts[lane * G + g];
+        uint32_t sum = c;
+        for (uint32_t o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += u;
+        }
+        counts[lane * G + g] = sum - c;
+        if (lane == 31) totals[g] = sum;
     }
+    __syncthreads();
+    // where each group and its tiles start: two groups to a thread
+    uint32_t total[2], rows_before = 0, tiles_before = 0;
+    for (uint32_t j = 0; j < 2; j++) total[j] = 2 * threadIdx.x + j < G ? totals[2 * threadIdx.x + j] : 0;
     uint32_t r = total[0] + total[1], n = (total[0] + TM - 1) / TM + (total[1] + TM - 1) / TM;
     const uint32_t own_r = r, own_n = n;
     for (uint32_t o = 1; o < 32; o <<= 1) {
@@ -212,33 +295,82 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
     for (uint32_t j = 0; j < 2; j++) {
         const uint32_t g = 2 * threadIdx.x + j;
         if (g >= G) break;
-        for (uint32_t w = 0; w < 32; w++) counts[w * G + g] += rows_before;
+        totals[g] = rows_before;
         offsets[g] = rows_before;
         for (uint32_t at = 0; at < total[j]; at += TM) tiles[tiles_before++] = ATile{g, rows_before + at, min(TM, total[j] - at), 0};
         rows_before += total[j];
         if (g == S) { offsets[G] = rows_before; *n_tiles = tiles_before; }
     }
     __syncthreads();
-    for (uint32_t t = first + lane; t - lane < end; t += 32) {
-        uint32_t s = 0xffffffffu;
-        if (t < end) s = min(ids[t], S);
-        const uint32_t same = __match_any_sync(0xffffffffu, s);
-        uint32_t at = 0;
-        if (t < end) at = mine[s];
-        __syncwarp();
-        if (t < end) {
-            order[at + __popc(same & ((1u << lane) - 1))] = t;
-            if (__ffs(same) - 1 == (int)lane) mine[s] = at + __popc(same);
+    if (per > 32 * AHEAD) fetch(first);                      // else they are still there
+    for (uint32_t t0 = first; t0 < end; t0 += 32 * AHEAD) {
+        if (t0 != first) fetch(t0);
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; i++) {
+            if (t0 + 32 * i >= end) break;
+            const bool there = t0 + 32 * i + lane < end;
+            const uint32_t g = there ? min(s[i], S) : 0xffffffffu, same = __match_any_sync(0xffffffffu, g);
+            const uint32_t at = there ? mine[g] : 0;
+            __syncwarp();
+            if (there) {
+                order[totals[g] + at + __popc(same & ((1u << lane) - 1))] = t0 + 32 * i + lane;
+                if (__ffs(same) - 1 == (int)lane) mine[g] = at + __popc(same);
+            }
+            __syncwarp();
         }
-        __syncwarp();
     }
 }
 
 // ---- accumulators ---------------------------------------------------------------------------------------------------------
+// An accumulator loses up to a bit's weight at every instruction that adds to it (additions in the tensor core truncate), always towards
+// zero, so what counts is how many add to the same one.  Products of the leading planes go to MAINS accumulators in turn, and
+// the corrections, 2^-8 of them and less, to one of their own (`side`), where their truncations are as much smaller; the sums meet
+// in FP32 when they are read.  With all six products in one accumulator dA of 8192 tokens was 5.9e-6 off, as the plain form in FP32 is
+// 0.9e-6.  Two of the leading planes where that leaves the TMEM columns of three CTAs to an SM.
 template <uint32_t RP> struct Sums {
-    static constexpr uint32_t MAINS = RP <= 64 ? 2 : 1, SIDE = MAINS * RP, NEED = SIDE + RP;
+    static constexpr uint32_t MAINS = RP <= 32 ? 2 : 1, SIDE = MAINS * RP, NEED = SIDE + RP;
     static constexpr uint32_t COLS = NEED <= 64 ? 64 : NEED <= 128 ? 128 : 256;                      // TMEM is handed out in powers of two
+    static constexpr uint32_t CTAS = COLS <= 128 ? 3 : 2;    // to an SM
 };
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+// The MMAs of one step: every sixteen of K, every pair of planes.
+// One warp walks this, and one of its threads issues.  Whatever an instruction names has to be warp-uniform for the compiler as well (read
+// from shared memory it is not, out of a reduction it is): otherwise every operand is moved to a uniform register first, and an
+// instruction costs 87 cycles instead of 49 (N = 64) or 65 (N = 128; the same with and without a swizzle, K- and MN-major).
+template <typename TA, typename TB, int PA, int PB, bool AMN, bool BMN, uint32_t MAINS, uint32_t K16S>
+__device__ __forceinline__ void step_mma(uint32_t d, uint32_t d_step, uint32_t side, uint32_t a_at, uint32_t b_at, uint32_t idesc, bool first, uint32_t leader) {
+    const uint64_t a = TA::desc(a_at, AMN), b = TB::desc(b_at, BMN);
+    const uint32_t more = first ? 0 : 1;
+    if (!leader) return;
+    bool begun = false;
+#pragma unroll
+    for (int order = 2; order > 0; order--)                  // the smallest first
+#pragma unroll
+        for (uint32_t k = 0; k < K16S; k++)
+#pragma unroll
+            for (int i = 0; i < PA; i++) {
+                const int j = order - i;
+                if (j < 0 || j >= PB) continue;
+                tc_mma(side, a + ((i * TA::PLANE + k * TA::k16(AMN)) >> 4), b + ((j * TB::PLANE + k * TB::k16(BMN)) >> 4), idesc, begun ? 1 : more);
+                begun = true;
+            }
+#pragma unroll
+    for (uint32_t k = 0; k < K16S; k++)
+        tc_mma(d + k % MAINS * d_step, a + (k * TA::k16(AMN) >> 4), b + (k * TB::k16(BMN) >> 4), idesc, d_step == 0 || k >= MAINS ? 1 : more);
+}
+// Sixteen columns of a sum that lies in the accumulators of shrink and outer.
+template <uint32_t RP> __device__ __forceinline__ void load_sum(uint32_t addr, float (&v)[16]) {
+    float u[16];
+    tc_load16(addr, v);
+#pragma unroll
+    for (uint32_t m = 1; m <= Sums<RP>::MAINS; m++) {
+        tc_load16(addr + m * RP, u);
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] += u[i];
+    }
+}
 
 // ---- shrink -----------------------------------------------------------------------------------------------------------------
 struct Lists { const uint32_t *order, *offsets; const ATile *tiles; const uint32_t *n_tiles; };
@@ -247,7 +379,7 @@ template <typename W> struct ShrinkJob {
     Mat<W> w;
     const float *x;
     uint64_t pitch;
-    bool x_wide, w_wide;                                     // rows on boundaries of four values
+    bool x_fours;                                            // rows on boundaries of four values, no more than 2^32 such runs
     __nv_bfloat16 *planes;                                   // [3][rows][RP]: the result cut in three, rows in the lists' order
 };
 template <typename W> struct ShrinkArgs {
@@ -260,55 +392,16 @@ template <typename W> struct ShrinkArgs {
 };
 
 template <typename W, uint32_t RP> struct ShrinkMap {
-    static constexpr int WP = Four<W>::PLANES;
-    using X = Tile<TM, KC, 3>;
-    using WideW = Tile<RP, KC, WP>;                          // rows r, columns of the wide axis: K-major
-    using TallW = Tile<KC, RP, WP>;                          // rows of the wide axis, columns r: MN-major
-    static constexpr uint32_t W_BYTES = WideW::BYTES > TallW::BYTES ? WideW::BYTES : TallW::BYTES;
-    static constexpr uint32_t STAGE = (X::BYTES + W_BYTES + 15) & ~15u;
-    static constexpr uint32_t ORDER = 64, STAGES_AT = ORDER + TM * 4;
-    static constexpr uint32_t TOTAL = STAGES_AT + 2 * STAGE;
+    using X = Tile<TM, KC, 3>;                               // rows tokens: K-major
+    using Run = MatRun<W, RP, KC>;                           // Wide: K-major, Tall: MN-major
+    static constexpr uint32_t ORDER = 64, STAGE = ORDER + TM * 4, W_AT = STAGE + X::BYTES;
     static constexpr uint32_t PITCH = RP + 4;                // floats per row of the exchanged accumulators
-    static_assert(TM * PITCH * 4 <= 2 * STAGE, "accumulators fit the stages");
-    static constexpr uint32_t COLS = Sums<RP>::COLS;
+    static constexpr uint32_t END = W_AT + Run::BYTES, ACC_END = STAGE + TM * PITCH * 4, TOTAL = END > ACC_END ? END : ACC_END;
 };
 
-// An accumulator loses up to a bit's weight at every instruction that adds to it (additions in the tensor core truncate), always towards
-// zero, so what counts is how many add to the same one.  Products of the leading planes go to MAINS accumulators in turn, and
-// the corrections, 2^-8 of them and less, to one of their own (`side`), where their truncations are as much smaller; the sums meet
-// in FP32 when they are read.  With all six products in one accumulator dA of 8192 tokens was 5.9e-6 off, as the plain form in FP32 is
-// 0.9e-6.
-template <typename TA, typename TB, int PA, int PB, bool AMN, bool BMN, uint32_t MAINS>
-__device__ __forceinline__ void step_mma(uint32_t d, uint32_t d_step, uint32_t side, uint32_t a, uint32_t b, uint32_t idesc, uint32_t k16s, bool first, uint32_t leader) {
-    uint32_t accumulate = first ? 0 : 1;
-#pragma unroll
-    for (int order = 2; order > 0; order--)                  // the smallest first
-        for (uint32_t k = 0; k < k16s; k++)
-#pragma unroll
-            for (int i = 0; i < PA; i++) {
-                const int j = order - i;
-                if (j < 0 || j >= PB) continue;
-                if (leader) tc_mma(side, TA::desc(a + i * TA::PLANE + k * TA::k16(AMN), AMN), TB::desc(b + j * TB::PLANE + k * TB::k16(BMN), BMN), idesc, accumulate);
-                accumulate = 1;
-            }
-    for (uint32_t k = 0; k < k16s; k++) {
-        const uint32_t to = d + k % MAINS * d_step;
-        if (leader) tc_mma(to, TA::desc(a + k * TA::k16(AMN), AMN), TB::desc(b + k * TB::k16(BMN), BMN), idesc, to == side || !first || k >= MAINS);
-    }
-}
-// Sixteen columns of a sum that lies in the accumulators of shrink and outer.
-template <uint32_t RP, uint32_t MAINS> __device__ __forceinline__ void load_sum(uint32_t addr, float (&v)[16]) {
-    float u[16];
-    tc_load16(addr, v);
-#pragma unroll
-    for (uint32_t m = 1; m <= MAINS; m++) {
-        tc_load16(addr + m * RP, u);
-#pragma unroll
-        for (int i = 0; i < 16; i++) v[i] += u[i];
-    }
-}
+// One operand stage and no second one: three CTAs to an SM cover each other's waits, and two stages would leave room for one or two.
 template <typename W, uint32_t RP>
-__global__ void __launch_bounds__(THREADS) adapter_shrink_kernel(const __grid_constant__ ShrinkArgs<W> a) {
+__global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel(const __grid_constant__ ShrinkArgs<W> a) {
     namespace cg = cooperative_groups;
     using M = ShrinkMap<W, RP>;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -319,81 +412,69 @@ __global__ void __launch_bounds__(THREADS) adapter_shrink_kernel(const __grid_co
     const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank();
     grid_wait();
     grid_go();
-    const uint32_t tile = blockIdx.y;
-    if (tile >= *a.lists.n_tiles) return;                    // the same for all CTAs of a cluster
-    const ATile t = a.lists.tiles[tile];
+    if (blockIdx.y >= *a.lists.n_tiles) return;              // the same for all CTAs of a cluster
+    const ATile t = a.lists.tiles[blockIdx.y];
     if (t.slot >= a.slots) return;
-    const uint32_t rank = job.w.rank;
-    if (tid < 2) bar_init(base + 8 * tid);
-    if (warp == 0) tc_alloc(base + 32, M::COLS);
-    if (tid < TM) order[tid] = tid < t.rows ? a.lists.order[t.first + tid] : 0;
+    if (tid == 0) bar_init(base);
+    if (warp == 0) tc_alloc(base + 32, Sums<RP>::COLS);
+    if (tid < TM) order[tid] = a.lists.order[t.first + min(tid, t.rows - 1)];      // rows that are not there: the last one again, unused
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = *(volatile uint32_t *)(smem + 32);
-    const uint64_t width = job.w.width;
-    const uint64_t per = ((width + parts - 1) / parts + KC - 1) / KC * KC, c_first = min(width, part * per), c_end = min(width, c_first + per);
-    const uint32_t steps = (uint32_t)((c_end - c_first + KC - 1) / KC);
-    const W *w = job.w.p + t.slot * job.w.slot;
+    const uint32_t tmem = uniform(*(volatile uint32_t *)(smem + 32));
+    const Mat<W> m = job.w;
+    const uint32_t per = ((m.width + parts - 1) / parts + KC - 1) / KC * KC, c_first = min(m.width, part * per), c_end = min(m.width, c_first + per);
+    const uint32_t steps = uniform((c_end - c_first + KC - 1) / KC);
+    const W *w = m.p + t.slot * m.slot;
 
-    constexpr uint32_t XU = TM * KC / 4 / THREADS, WU = RP * KC / 4 / THREADS;       // runs of four values per thread
-    Four<float> xv[XU];
-    Four<W> wv[WU];
+    constexpr uint32_t XU = TM * KC / 4 / THREADS, ROWS = THREADS / (KC / 4);        // runs of four values per thread, rows from one to the next
     const uint32_t x_row = tid / (KC / 4), x_col = tid % (KC / 4) * 4;
-    auto fetch = [&](uint64_t c0) {
+    Four<float> xv[XU];
+    uint32_t x_at[XU];                                       // places in runs of four
+    typename M::Run wv;
 #pragma unroll
-        for (uint32_t i = 0; i < XU; i++) {
-            const uint32_t row = x_row + i * (THREADS / (KC / 4));
-            if (row < t.rows) xv[i].load(job.x + order[row] * job.pitch + c0 + x_col, (int)min((uint64_t)4, c_end - min(c_end, c0 + x_col)), job.x_wide);
-        }
+    for (uint32_t i = 0; i < XU; i++) x_at[i] = (uint32_t)((order[x_row + i * ROWS] * job.pitch + c_first + x_col) / 4);
+    wv.begin(m, c_first);
+    const float *x = job.x;
+    auto fetch = [&](uint32_t c0) {
+        if (job.x_fours && c0 + KC <= c_end) {
 #pragma unroll
-        for (uint32_t i = 0; i < WU; i++) {
-            const uint32_t u = tid + i * THREADS;
-            if (job.w.wide) {
-                const uint32_t r = u / (KC / 4);
-                const uint64_t c = c0 + u % (KC / 4) * 4;
-                wv[i].load(w + r * width + c, r < rank ? (int)min((uint64_t)4, c_end - min(c_end, c)) : 0, job.w_wide);
-            } else {
-                const uint64_t c = c0 + u / (RP / 4);
-                const uint32_t r = u % (RP / 4) * 4;
-                wv[i].load(w + c * rank + r, c < c_end ? (int)min(4u, rank - min(rank, r)) : 0, job.w_wide);
-            }
+            for (uint32_t i = 0; i < XU; i++) { xv[i].load4(x + (uint64_t)x_at[i] * 4); x_at[i] += KC / 4; }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < XU; i++) xv[i].load1(x + order[x_row + i * ROWS] * job.pitch, c0 + x_col, c_end - 1);
         }
+        wv.load(m, w, c0, c_end);
     };
     if (steps) fetch(c_first);
-    const uint32_t idesc = idesc_of(TM, RP, false, !job.w.wide);
+    const uint32_t idesc = idesc_of(TM, RP, false, !m.wide);
     for (uint32_t s = 0; s < steps; s++) {
-        const uint32_t at = base + M::STAGES_AT + (s & 1) * M::STAGE, wat = at + M::X::BYTES;
-        if (s >= 2) bar_wait(base + 8 * (s & 1), (s / 2 - 1) & 1, a.status);
+        const uint32_t c0 = c_first + s * KC;
+        if (s) bar_wait(base, (s - 1) & 1, a.status);
+        if (c0 + KC > c_end)
 #pragma unroll
-        for (uint32_t i = 0; i < XU; i++) {
-            const uint32_t row = x_row + i * (THREADS / (KC / 4));
-            if (row < t.rows) xv[i].put(at + M::X::at(row, x_col), M::X::PLANE);
-        }
+            for (uint32_t i = 0; i < XU; i++) xv[i].keep(places(c0 + x_col, c_end));
 #pragma unroll
-        for (uint32_t i = 0; i < WU; i++) {
-            const uint32_t u = tid + i * THREADS;
-            if (job.w.wide) wv[i].put(wat + M::WideW::at(u / (KC / 4), u % (KC / 4) * 4), M::WideW::PLANE);
-            else wv[i].put(wat + M::TallW::at(u / (RP / 4), u % (RP / 4) * 4), M::TallW::PLANE);
-        }
-        if (s + 1 < steps) fetch(c_first + (uint64_t)(s + 1) * KC);
+        for (uint32_t i = 0; i < XU; i++) xv[i].put(base + M::STAGE + M::X::at(x_row + i * ROWS, x_col), M::X::PLANE);
+        wv.put(m, c0, c_end, base + M::W_AT);
+        if (s + 1 < steps) fetch(c0 + KC);
         fence_async();
         __syncthreads();
         if (warp == 0) {
             tc_after();
             const uint32_t leader = elect();                 // the thread whose products the commit answers for
-            if (job.w.wide) step_mma<typename M::X, typename M::WideW, 3, M::WP, false, false, Sums<RP>::MAINS>(tmem, RP, tmem + Sums<RP>::SIDE, at, wat, idesc, KC / 16, s == 0, leader);
-            else step_mma<typename M::X, typename M::TallW, 3, M::WP, false, true, Sums<RP>::MAINS>(tmem, RP, tmem + Sums<RP>::SIDE, at, wat, idesc, KC / 16, s == 0, leader);
-            if (leader) tc_commit(base + 8 * (s & 1));
+            if (m.wide) step_mma<typename M::X, typename M::Run::Wide, 3, M::Run::PLANES, false, false, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::W_AT, idesc, s == 0, leader);
+            else step_mma<typename M::X, typename M::Run::Tall, 3, M::Run::PLANES, false, true, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::W_AT, idesc, s == 0, leader);
+            if (leader) tc_commit(base);
         }
     }
-    if (steps) bar_wait(base + 8 * ((steps - 1) & 1), ((steps - 1) / 2) & 1, a.status);
+    if (steps) bar_wait(base, (steps - 1) & 1, a.status);
     tc_after();
     // accumulators to shared memory, summed over the cluster's CTAs in their order, scaled, cut and stored
-    float *acc = (float *)(smem + M::STAGES_AT);
+    float *acc = (float *)(smem + M::STAGE);
     for (uint32_t c = (warp >> 2) * 16; c < RP; c += 32) {
         float v[16];
-        load_sum<RP, Sums<RP>::MAINS>(tmem + ((warp & 3) << 21) + c, v);
+        load_sum<RP>(tmem + ((warp & 3) << 21) + c, v);
         float *row = acc + ((warp & 3) * 32 + lane) * M::PITCH + c;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) *(float4 *)(row + i) = steps ? make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_float4(0, 0, 0, 0);
@@ -401,7 +482,7 @@ __global__ void __launch_bounds__(THREADS) adapter_shrink_kernel(const __grid_co
     tc_before();
     cluster.sync();
     tc_after();
-    if (warp == 0) tc_free(tmem, M::COLS);
+    if (warp == 0) tc_free(tmem, Sums<RP>::COLS);
     const float scale = a.scale ? a.scale[t.slot] : 1.0f;
     const uint32_t rows = TM / parts;
     for (uint32_t u = tid; u < rows * (RP / 4); u += THREADS) {
@@ -425,7 +506,6 @@ __global__ void __launch_bounds__(THREADS) adapter_shrink_kernel(const __grid_co
 // ---- expand -----------------------------------------------------------------------------------------------------------------
 template <typename W> struct ExpandArgs {
     Mat<W> w;
-    bool w_wide;
     const __nv_bfloat16 *planes;                             // [3][rows][RP], of shrink
     uint64_t plane;
     Lists lists;
@@ -437,104 +517,99 @@ template <typename W> struct ExpandArgs {
     uint32_t *status;
 };
 template <typename W, uint32_t RP> struct ExpandMap {
-    static constexpr int WP = Four<W>::PLANES;
     using H = Tile<TM, RP, 3>;                               // rows tokens: K-major
-    using TallW = Tile<128, RP, WP>;                         // rows of the wide axis: K-major
-    using WideW = Tile<RP, 128, WP>;                         // rows r: MN-major
-    static constexpr uint32_t W_BYTES = WideW::BYTES > TallW::BYTES ? WideW::BYTES : TallW::BYTES;
-    static constexpr uint32_t ORDER = 64, H_AT = ORDER + TM * 4, W_AT = H_AT + ((H::BYTES + 15) & ~15u), NEED = W_AT + W_BYTES;
+    using Run = MatRun<W, RP, 128>;                          // Tall: K-major, Wide: MN-major
+    static constexpr uint32_t PLACES = 64, H_AT = PLACES + TM * 16, W_AT = H_AT + H::BYTES, NEED = W_AT + Run::BYTES;
     // Never more than four CTAs on an SM, which have its 512 columns of TMEM: a fifth would hold its place waiting for columns (233472
     // bytes of shared memory to an SM, 1024 of them the system's for each CTA).
-    static constexpr uint32_t TOTAL = NEED < 46080 ? 46080 : NEED;
+    static constexpr uint32_t TOTAL = NEED < 46080 ? 46080 : NEED, CTAS = TOTAL < 75000 ? 3 : TOTAL < 115000 ? 2 : 1;
     static_assert(5 * (TOTAL + 1024) > 233472 && TM == 128, "at most four CTAs of 128 TMEM columns");
 };
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Columns of the projection are the accumulator's lanes and tokens its columns, so that a warp's 32 lanes hold 32 neighbouring values
-// of a token's row.
+// of a token's row.  base is read a batch of sixteen rows ahead of the one that is added.
 template <typename W, uint32_t RP>
-__global__ void __launch_bounds__(THREADS) adapter_expand_kernel(const __grid_constant__ ExpandArgs<W> a) {
+__global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expand_kernel(const __grid_constant__ ExpandArgs<W> a) {
     using M = ExpandMap<W, RP>;
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, base = smem_u32(smem);
-    uint32_t *order = (uint32_t *)(smem + M::ORDER);
+    struct Place { uint64_t b, y; };                         // bytes from the first row of base and of y
+    Place *place = (Place *)(smem + M::PLACES);
     grid_wait();
     grid_go();
     if (blockIdx.y >= *a.lists.n_tiles) return;
     const ATile t = a.lists.tiles[blockIdx.y];
     const bool none = t.slot >= a.slots;
     if (none && a.base == a.y) return;
-    const uint64_t width = a.w.width;
-    const uint32_t rank = a.w.rank;
-    const uint32_t first = blockIdx.x * a.blocks, last = (uint32_t)min((width + 127) / 128, (uint64_t)first + a.blocks);
+    const Mat<W> m = a.w;
+    const uint32_t first = blockIdx.x * a.blocks, last = min((m.width + 127) / 128, first + a.blocks);
     if (tid == 0) bar_init(base);
     if (warp == 0) tc_alloc(base + 32, TM);
-    if (tid < TM) order[tid] = tid < t.rows ? a.lists.order[t.first + tid] : 0;
-    const W *w = a.w.p + t.slot * a.w.slot;
-    constexpr uint32_t WU = RP * 128 / 4 / THREADS;
-    Four<W> wv[WU];
-    auto fetch = [&](uint32_t block) {
-        const uint64_t c0 = (uint64_t)block * 128;
-#pragma unroll
-        for (uint32_t i = 0; i < WU; i++) {
-            const uint32_t u = tid + i * THREADS;
-            if (a.w.wide) {
-                const uint32_t r = u / 32;
-                const uint64_t c = c0 + u % 32 * 4;
-                wv[i].load(w + r * width + c, r < rank ? (int)min((uint64_t)4, width - min(width, c)) : 0, a.w_wide);
-            } else {
-                const uint64_t c = c0 + u / (RP / 4);
-                const uint32_t r = u % (RP / 4) * 4;
-                wv[i].load(w + c * rank + r, c < width ? (int)min(4u, rank - min(rank, r)) : 0, a.w_wide);
-            }
-        }
-    };
-    const uint32_t n = (t.rows + 15) & ~15u;
+    if (tid < TM) {
+        const uint64_t row = a.lists.order[t.first + min(tid, t.rows - 1)];
+        place[tid] = Place{row * a.base_pitch * 4, row * a.y_pitch * 4};
+    }
+    const W *w = m.p + t.slot * m.slot;
+    typename M::Run wv;
+    const uint32_t n = uniform((t.rows + 15) & ~15u);
     if (!none) {
-        fetch(first);
         for (uint32_t u = tid; u < 3 * t.rows * (RP / 8); u += THREADS) {
             const uint32_t p = u / (t.rows * (RP / 8)), v = u % (t.rows * (RP / 8)), row = v / (RP / 8), c = v % (RP / 8) * 8;
-            put16(base + M::H_AT + p * M::H::PLANE + M::H::at(row, c), *(const uint4 *)(a.planes + p * a.plane + (uint64_t)(t.first + row) * RP + c));
+            copy16(base + M::H_AT + p * M::H::PLANE + M::H::at(row, c), a.planes + p * a.plane + (uint64_t)(t.first + row) * RP + c);
         }
+        wv.begin(m, first * 128);
+        wv.load(m, w, first * 128, m.width);
+        copies_done();
     }
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = *(volatile uint32_t *)(smem + 32);
-    const uint32_t idesc = idesc_of(128, n, a.w.wide, false);
+    const uint32_t tmem = uniform(*(volatile uint32_t *)(smem + 32));
+    const uint32_t idesc = idesc_of(128, n, m.wide, false);
+    const uint32_t t_first = (warp >> 2) * 64, t_last = min(t.rows, t_first + 64), d = tmem + ((warp & 3) << 21);
+    const bool added = a.base != nullptr;
     for (uint32_t block = first; block < last; block++) {
-        if (!none) {
+        const uint32_t c = block * 128 + (warp & 3) * 32 + lane;
+        const char *b_col = (const char *)(a.base + min(c, m.width - 1));
+        char *y_col = (char *)(a.y + c);
+        float b[16], v[16];
+        auto fetch = [&](uint32_t j) {
 #pragma unroll
-            for (uint32_t i = 0; i < WU; i++) {
-                const uint32_t u = tid + i * THREADS;
-                if (a.w.wide) wv[i].put(base + M::W_AT + M::WideW::at(u / 32, u % 32 * 4), M::WideW::PLANE);
-                else wv[i].put(base + M::W_AT + M::TallW::at(u / (RP / 4), u % (RP / 4) * 4), M::TallW::PLANE);
-            }
-            if (block + 1 < last) fetch(block + 1);
+            for (uint32_t i = 0; i < 16; i++) b[i] = *(const float *)(b_col + place[j + i].b);
+        };
+        if (added && t_first < t_last) fetch(t_first);
+        if (!none) {
+            wv.put(m, block * 128, m.width, base + M::W_AT);
+            if (block + 1 < last) wv.load(m, w, (block + 1) * 128, m.width);
             fence_async();
             tc_before();
             __syncthreads();
             if (warp == 0) {
                 tc_after();
                 const uint32_t leader = elect();
-                if (a.w.wide) step_mma<typename M::WideW, typename M::H, M::WP, 3, true, false, 1>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, RP / 16, true, leader);
-                else step_mma<typename M::TallW, typename M::H, M::WP, 3, false, false, 1>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, RP / 16, true, leader);
+                if (m.wide) step_mma<typename M::Run::Wide, typename M::H, M::Run::PLANES, 3, true, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
+                else step_mma<typename M::Run::Tall, typename M::H, M::Run::PLANES, 3, false, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
                 if (leader) tc_commit(base);
             }
+            bar_wait(base, (block - first) & 1, a.status);
+            tc_after();
         }
-        const uint64_t c = (uint64_t)block * 128 + (warp & 3) * 32 + lane;
-        const bool mine = c < width;
-        const uint32_t t_first = (warp >> 2) * 64, t_last = min(t.rows, t_first + 64);
-        bool waited = none;
         for (uint32_t j = t_first; j < t_last; j += 16) {
-            float b[16], v[16];
+            if (none) {
 #pragma unroll
-            for (uint32_t i = 0; i < 16; i++) b[i] = a.base && mine && j + i < t_last ? a.base[order[j + i] * a.base_pitch + c] : 0.0f;
-            if (!waited) { bar_wait(base, (block - first) & 1, a.status); tc_after(); waited = true; }
-            if (!none) tc_load16(tmem + ((warp & 3) << 21) + j, v);
+                for (uint32_t i = 0; i < 16; i++) v[i] = 0;
+            } else tc_load16(d + j, v);
+            if (added)
 #pragma unroll
-            for (uint32_t i = 0; i < 16; i++) if (mine && j + i < t_last) a.y[order[j + i] * a.y_pitch + c] = none ? b[i] : b[i] + v[i];
+                for (uint32_t i = 0; i < 16; i++) v[i] = none ? b[i] : b[i] + v[i];
+            if (added && j + 16 < t_last) fetch(j + 16);
+            if (c < m.width)
+#pragma unroll
+                for (uint32_t i = 0; i < 16; i++) if (j + i < t_last) *(float *)(y_col + place[j + i].y) = v[i];
         }
-        if (!waited) bar_wait(base, (block - first) & 1, a.status);          // the tile's columns of weights are written again only then
     }
     tc_before();
     __syncthreads();
@@ -544,11 +619,12 @@ __global__ void __launch_bounds__(THREADS) adapter_expand_kernel(const __grid_co
 // ---- outer ------------------------------------------------------------------------------------------------------------------
 struct OuterJob {
     const float *x;
-    uint64_t pitch, width;
-    bool x_wide;
+    uint64_t pitch;
+    uint32_t width;
+    bool x_fours;
     const __nv_bfloat16 *planes;                             // [3][rows][RP]
     float *d;                                                // [slots][rank * width]: (r, c) at r * sr + c * sc
-    uint64_t sr, sc;
+    uint32_t sr, sc;
     uint32_t blocks;                                         // of 128 columns
 };
 struct OuterArgs {
@@ -561,15 +637,13 @@ struct OuterArgs {
 template <uint32_t RP> struct OuterMap {
     using X = Tile<TC, 128, 3>;                              // rows tokens: MN-major
     using H = Tile<TC, RP, 3>;                               // rows tokens: MN-major
-    static constexpr uint32_t STAGE = (X::BYTES + H::BYTES + 15) & ~15u, STAGES_AT = 64;
+    static constexpr uint32_t STAGE = 64, H_AT = STAGE + X::BYTES, END = H_AT + H::BYTES;
     static constexpr uint32_t PITCH = 129;                   // floats per r of the exchanged accumulators
-    static constexpr uint32_t ACC = RP * PITCH * 4;
-    static constexpr uint32_t TOTAL = STAGES_AT + (2 * STAGE > ACC ? 2 * STAGE : ACC);
-    static constexpr uint32_t COLS = Sums<RP>::COLS;
+    static constexpr uint32_t ACC_END = STAGE + RP * PITCH * 4, TOTAL = END > ACC_END ? END : ACC_END;
 };
 
 template <uint32_t RP>
-__global__ void __launch_bounds__(THREADS) adapter_outer_kernel(const __grid_constant__ OuterArgs a) {
+__global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(const __grid_constant__ OuterArgs a) {
     namespace cg = cooperative_groups;
     using M = OuterMap<RP>;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -578,82 +652,84 @@ __global__ void __launch_bounds__(THREADS) adapter_outer_kernel(const __grid_con
     const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank(), slot = blockIdx.z;
     const bool second = blockIdx.y >= a.job[0].blocks;
     const OuterJob &job = a.job[second];
-    const uint64_t c0 = (uint64_t)(blockIdx.y - (second ? a.job[0].blocks : 0)) * 128;
+    const uint32_t c0 = (blockIdx.y - (second ? a.job[0].blocks : 0)) * 128;
     grid_wait();
     grid_go();
     const uint32_t begin = a.lists.offsets[slot], tokens = a.lists.offsets[slot + 1] - begin;
-    const uint32_t cols = (uint32_t)min((uint64_t)128, job.width - c0);
-    float *d = job.d + slot * (a.rank * job.width) + c0 * job.sc;
+    const uint32_t cols = min(128u, job.width - c0), sr = job.sr, sc = job.sc;
+    float *d = job.d + (uint64_t)slot * a.rank * job.width + c0 * sc;
     if (!tokens) {
-        for (uint32_t u = part * THREADS + tid; u < a.rank * cols; u += parts * THREADS)
-            d[job.sc == 1 ? u / cols * job.sr + u % cols : u % a.rank * job.sr + u / a.rank * job.sc] = 0;
+        for (uint32_t u = part * THREADS + tid; u < a.rank * cols; u += parts * THREADS) d[sc == 1 ? u / cols * sr + u % cols : u % a.rank * sr + u / a.rank * sc] = 0;
         return;                                              // the same for all CTAs of the cluster
     }
-    if (tid < 2) bar_init(base + 8 * tid);
-    if (warp == 0) tc_alloc(base + 32, M::COLS);
+    if (tid == 0) bar_init(base);
+    if (warp == 0) tc_alloc(base + 32, Sums<RP>::COLS);
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = *(volatile uint32_t *)(smem + 32);
+    const uint32_t tmem = uniform(*(volatile uint32_t *)(smem + 32));
     const uint32_t per = ((tokens + parts - 1) / parts + TC - 1) / TC * TC, from = min(tokens, part * per), to = min(tokens, from + per);
-    const uint32_t steps = (to - from + TC - 1) / TC;
-    constexpr uint32_t XU = TC * 128 / 4 / THREADS, HU = (3 * TC * RP / 8 + THREADS - 1) / THREADS;
-    Four<float> xv[XU];
-    uint4 hv[HU];
+    const uint32_t steps = uniform((to - from + TC - 1) / TC);
+    constexpr uint32_t XU = TC * 128 / 4 / THREADS, HU = TC * RP / 8;
     const uint32_t x_row = tid / 32, x_col = lane * 4;
-    auto fetch = [&](uint32_t t0) {
+    const float *x = job.x + c0;
+    Four<float> xv[XU];
+    uint32_t ids[XU];                                        // tokens of the step after the one that is fetched
+    auto fetch_ids = [&](uint32_t t0) {
 #pragma unroll
-        for (uint32_t i = 0; i < XU; i++) {
-            const uint32_t t = t0 + x_row + i * 8;
-            const int valid = t < to ? (int)cols - (int)x_col : 0;
-            xv[i].load(valid > 0 ? job.x + a.lists.order[begin + t] * job.pitch + c0 + x_col : nullptr, valid, job.x_wide);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < HU; i++) {
-            const uint32_t u = tid + i * THREADS, p = u / (TC * RP / 8), v = u % (TC * RP / 8), t = t0 + v / (RP / 8);
-            hv[i] = p < 3 && t < to ? *(const uint4 *)(job.planes + p * a.plane + (uint64_t)(begin + t) * RP + v % (RP / 8) * 8) : make_uint4(0, 0, 0, 0);
-        }
+        for (uint32_t i = 0; i < XU; i++) ids[i] = a.lists.order[begin + min(t0 + x_row + i * 8, to - 1)];
     };
-    if (steps) fetch(from);
+    auto fetch = [&](uint32_t t0) {
+        if (job.x_fours && cols == 128) {
+#pragma unroll
+            for (uint32_t i = 0; i < XU; i++) xv[i].load4(x + ids[i] * job.pitch + x_col);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < XU; i++) xv[i].load1(x + ids[i] * job.pitch, x_col, cols - 1);
+        }
+        if (t0 + TC < to) fetch_ids(t0 + TC);
+    };
+    if (steps) { fetch_ids(from); fetch(from); }
     constexpr uint32_t idesc = idesc_of(128, RP, true, true);
     for (uint32_t s = 0; s < steps; s++) {
-        const uint32_t at = base + M::STAGES_AT + (s & 1) * M::STAGE, hat = at + M::X::BYTES;
-        if (s >= 2) bar_wait(base + 8 * (s & 1), (s / 2 - 1) & 1, a.status);
-#pragma unroll
-        for (uint32_t i = 0; i < XU; i++) xv[i].put(at + M::X::at(x_row + i * 8, x_col), M::X::PLANE);
-#pragma unroll
-        for (uint32_t i = 0; i < HU; i++) {
-            const uint32_t u = tid + i * THREADS, p = u / (TC * RP / 8), v = u % (TC * RP / 8);
-            if (p < 3) put16(hat + p * M::H::PLANE + M::H::at(v / (RP / 8), v % (RP / 8) * 8), hv[i]);
+        const uint32_t t0 = from + s * TC;
+        if (s) bar_wait(base, (s - 1) & 1, a.status);
+        for (uint32_t u = tid; u < 3 * HU; u += THREADS) {   // out of L2, under the cutting of x
+            const uint32_t p = u / HU, v = u % HU, row = v / (RP / 8), c = v % (RP / 8) * 8, to_at = base + M::H_AT + p * M::H::PLANE + M::H::at(row, c);
+            if (t0 + row < to) copy16(to_at, job.planes + p * a.plane + (uint64_t)(begin + t0 + row) * RP + c);
+            else put16(to_at, make_uint4(0, 0, 0, 0));       // a token that is not there adds nothing
         }
-        if (s + 1 < steps) fetch(from + (s + 1) * TC);
+#pragma unroll
+        for (uint32_t i = 0; i < XU; i++) xv[i].put(base + M::STAGE + M::X::at(x_row + i * 8, x_col), M::X::PLANE);
+        if (s + 1 < steps) fetch(t0 + TC);
+        copies_done();
         fence_async();
         __syncthreads();
         if (warp == 0) {
             tc_after();
             const uint32_t leader = elect();
-            step_mma<typename M::X, typename M::H, 3, 3, true, true, Sums<RP>::MAINS>(tmem, RP, tmem + Sums<RP>::SIDE, at, hat, idesc, TC / 16, s == 0, leader);
-            if (leader) tc_commit(base + 8 * (s & 1));
+            step_mma<typename M::X, typename M::H, 3, 3, true, true, Sums<RP>::MAINS, TC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::H_AT, idesc, s == 0, leader);
+            if (leader) tc_commit(base);
         }
     }
-    if (steps) bar_wait(base + 8 * ((steps - 1) & 1), ((steps - 1) / 2) & 1, a.status);
+    if (steps) bar_wait(base, (steps - 1) & 1, a.status);
     tc_after();
-    float *acc = (float *)(smem + M::STAGES_AT);
+    float *acc = (float *)(smem + M::STAGE);
     for (uint32_t c = (warp >> 2) * 16; c < RP; c += 32) {
         float v[16];
-        load_sum<RP, Sums<RP>::MAINS>(tmem + ((warp & 3) << 21) + c, v);
+        load_sum<RP>(tmem + ((warp & 3) << 21) + c, v);
 #pragma unroll
         for (uint32_t i = 0; i < 16; i++) acc[(c + i) * M::PITCH + (warp & 3) * 32 + lane] = steps ? v[i] : 0.0f;
     }
     tc_before();
     cluster.sync();
     tc_after();
-    if (warp == 0) tc_free(tmem, M::COLS);
+    if (warp == 0) tc_free(tmem, Sums<RP>::COLS);
     for (uint32_t u = part * THREADS + tid; u < a.rank * cols; u += parts * THREADS) {
-        const uint32_t r = job.sc == 1 ? u / cols : u % a.rank, c = job.sc == 1 ? u % cols : u / a.rank;
+        const uint32_t r = sc == 1 ? u / cols : u % a.rank, c = sc == 1 ? u % cols : u / a.rank;
         float sum = 0;
         for (uint32_t p = 0; p < parts; p++) sum += cluster.map_shared_rank(acc, p)[r * M::PITCH + c];
-        d[r * job.sr + c * job.sc] = sum;
+        d[r * sr + c * sc] = sum;
     }
     cluster.sync();
 }
@@ -690,7 +766,7 @@ int make_lists(const QW4ShTune *tune, const QW4CuAdapters *ad, const uint32_t *s
     s.tiles = (uint32_t)qw4sh_adapter_tiles(T, s.S);
     s.lists = {tune->order, tune->offsets, (const ATile *)tune->tiles, tune->n_tiles};
     s.scale = ad->scale; s.status = tune->status; s.plane = (uint64_t)T * s.RP; s.stream = stream;
-    return launch(adapter_lists_kernel, "adapter_lists_kernel", dim3(1), 1024, (size_t)32 * (s.S + 1) * 4, 0, false, stream, slots, s.T, s.S, tune->order,
+    return launch(adapter_lists_kernel, "adapter_lists_kernel", dim3(1), 1024, (size_t)33 * (s.S + 1) * 4, 0, false, stream, slots, s.T, s.S, tune->order,
                   tune->offsets, (ATile *)tune->tiles, tune->n_tiles, tune->status);
 }
 
@@ -711,8 +787,8 @@ int shrink(const ShrinkJob<W> *jobs, uint32_t n, const Shape &s) {
     return launch(adapter_shrink_kernel<W, RP>, "adapter_shrink_kernel", dim3(c, s.tiles, n), THREADS, ShrinkMap<W, RP>::TOTAL, c, true, s.stream, a);
 }
 template <typename W, uint32_t RP>
-int expand(const Mat<W> &w, bool w_wide, const __nv_bfloat16 *planes, const float *base, size_t base_pitch, float *y, size_t y_pitch, const Shape &s) {
-    ExpandArgs<W> a = {w, w_wide, planes, s.plane, s.lists, s.S, 1, base, base_pitch, y, y_pitch, s.status};
+int expand(const Mat<W> &w, const __nv_bfloat16 *planes, const float *base, size_t base_pitch, float *y, size_t y_pitch, const Shape &s) {
+    ExpandArgs<W> a = {w, planes, s.plane, s.lists, s.S, 1, base, base_pitch, y, y_pitch, s.status};
     const uint64_t blocks = (w.width + 127) / 128, tiles = (s.T + TM - 1) / TM;
     a.blocks = (uint32_t)((blocks * tiles + 3 * SMS - 1) / (3 * SMS));
     if (a.blocks > blocks) a.blocks = (uint32_t)blocks;
@@ -727,29 +803,28 @@ int outer(const OuterJob *jobs, const Shape &s) {
     return launch(adapter_outer_kernel<RP>, "adapter_outer_kernel", dim3(c, blocks, s.S), THREADS, OuterMap<RP>::TOTAL, c, true, s.stream, a);
 }
 
-template <typename W> Mat<W> mat_a(const QW4CuAdapters *ad) { return {(const W *)ad->a, ad->rank * ad->k, ad->rank, ad->k, true}; }
-template <typename W> Mat<W> mat_b(const QW4CuAdapters *ad) { return {(const W *)ad->b, ad->rank * ad->n, ad->rank, ad->n, false}; }
-template <typename W> bool wide_a(const QW4CuAdapters *ad) { return fours(ad->a, ad->k, sizeof(W)); }
-template <typename W> bool wide_b(const QW4CuAdapters *ad) { return fours(ad->b, ad->rank, sizeof(W)); }
+template <typename W> Mat<W> mat_a(const QW4CuAdapters *ad) { return {(const W *)ad->a, ad->rank * ad->k, ad->rank, (uint32_t)ad->k, true, fours(ad->a, ad->k, sizeof(W))}; }
+template <typename W> Mat<W> mat_b(const QW4CuAdapters *ad) { return {(const W *)ad->b, ad->rank * ad->n, ad->rank, (uint32_t)ad->n, false, fours(ad->b, ad->rank, sizeof(W))}; }
 
 struct Rows { const float *p; size_t pitch; };
+bool runs(Rows x, uint64_t T) { return fours(x.p, x.pitch, 4) && T * x.pitch < 1ull << 34; }
 
 template <typename W, uint32_t RP>
 int forward(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, Rows base, float *y, size_t y_pitch, const Shape &s) {
-    const ShrinkJob<W> job = {mat_a<W>(ad), x.p, x.pitch, fours(x.p, x.pitch, 4), wide_a<W>(ad), (__nv_bfloat16 *)tune->h};
+    const ShrinkJob<W> job = {mat_a<W>(ad), x.p, x.pitch, runs(x, s.T), (__nv_bfloat16 *)tune->h};
     if (const int rc = shrink<W, RP>(&job, 1, s)) return rc;
-    return expand<W, RP>(mat_b<W>(ad), wide_b<W>(ad), job.planes, base.p, base.pitch, y, y_pitch, s);
+    return expand<W, RP>(mat_b<W>(ad), job.planes, base.p, base.pitch, y, y_pitch, s);
 }
 template <typename W, uint32_t RP>
 int backward(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, Rows dy, Rows base, float *dx, size_t dx_pitch, float *da, float *db, const Shape &s) {
-    const ShrinkJob<W> jobs[2] = {{mat_b<W>(ad), dy.p, dy.pitch, fours(dy.p, dy.pitch, 4), wide_b<W>(ad), (__nv_bfloat16 *)tune->g},
-                                  {mat_a<W>(ad), x.p, x.pitch, fours(x.p, x.pitch, 4), wide_a<W>(ad), (__nv_bfloat16 *)tune->h}};
+    const ShrinkJob<W> jobs[2] = {{mat_b<W>(ad), dy.p, dy.pitch, runs(dy, s.T), (__nv_bfloat16 *)tune->g},
+                                  {mat_a<W>(ad), x.p, x.pitch, runs(x, s.T), (__nv_bfloat16 *)tune->h}};
     int rc;
     if ((rc = shrink<W, RP>(jobs, da ? 2 : 1, s))) return rc;
-    if (dx && (rc = expand<W, RP>(mat_a<W>(ad), wide_a<W>(ad), jobs[0].planes, base.p, base.pitch, dx, dx_pitch, s))) return rc;
+    if (dx && (rc = expand<W, RP>(mat_a<W>(ad), jobs[0].planes, base.p, base.pitch, dx, dx_pitch, s))) return rc;
     if (!da) return 0;
-    const OuterJob outers[2] = {{x.p, x.pitch, ad->k, jobs[1].x_wide, jobs[0].planes, da, ad->k, 1, (uint32_t)((ad->k + 127) / 128)},
-                                {dy.p, dy.pitch, ad->n, jobs[0].x_wide, jobs[1].planes, db, 1, ad->rank, (uint32_t)((ad->n + 127) / 128)}};
+    const OuterJob outers[2] = {{x.p, x.pitch, (uint32_t)ad->k, jobs[1].x_fours, jobs[0].planes, da, (uint32_t)ad->k, 1, (uint32_t)((ad->k + 127) / 128)},
+                                {dy.p, dy.pitch, (uint32_t)ad->n, jobs[0].x_fours, jobs[1].planes, db, 1, ad->rank, (uint32_t)((ad->n + 127) / 128)}};
     return outer<RP>(outers, s);
 }
 
