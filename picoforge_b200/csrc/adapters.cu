@@ -100,10 +100,29 @@ template <uint32_t ROWS, uint32_t COLS, uint32_t PLANES> struct Tile {
     static __host__ __device__ constexpr uint32_t k16(bool mn) { return mn ? 256 : 2 * GROUP; }          // bytes to the next sixteen of K
 };
 
-__device__ __forceinline__ void put8(uint32_t addr, uint32_t a, uint32_t b) { asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory"); }
-__device__ __forceinline__ void put16(uint32_t addr, uint4 v) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+// The result of shrink, rows of RP values cut in three planes, lies in memory as it is read: core matrices of eight rows x eight values, the
+// matrices of eight rows behind one another.  A slot's rows start at a multiple of sixteen and end at one, zeros behind the
+// last, so a run of rows is one copy to a plane, and an operand with either axis as K.
+template <uint32_t ROWS, uint32_t RP> struct Rank {
+    static constexpr uint32_t PLANE = ROWS * RP * 2, BYTES = 3 * PLANE;
+    static __device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn) {
+        const uint32_t along_k = mn ? RP * 16 : 128, along_mn = mn ? 128 : RP * 16;
+        return (uint64_t)(addr >> 4 & 0x3fffu) | (uint64_t)(along_k >> 4) << 16 | (uint64_t)(along_mn >> 4) << 32 | 1ull << 46;
+    }
+    static __host__ __device__ constexpr uint32_t k16(bool mn) { return mn ? 2 * RP * 16 : 256; }
+};
+// Sixteen-row runs of its three planes to shared memory, by one thread; `bar` learns of their arrival.
+template <uint32_t ROWS, uint32_t RP>
+__device__ __forceinline__ void copy_rank(uint32_t dst, const __nv_bfloat16 *planes, uint64_t plane, uint32_t first, uint32_t rows16, uint32_t bar) {
+    const uint32_t bytes = rows16 * RP * 2;
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(3 * bytes) : "memory");
+#pragma unroll
+    for (uint32_t p = 0; p < 3; p++)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(dst + p * Rank<ROWS, RP>::PLANE), "l"(planes + p * plane + (uint64_t)first * RP), "r"(bytes), "r"(bar) : "memory");
 }
+
+__device__ __forceinline__ void put8(uint32_t addr, uint32_t a, uint32_t b) { asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory"); }
 
 // The upper sixteen bits of two values, and what they leave of them.
 __device__ __forceinline__ uint32_t cut2(float &a, float &b) {
@@ -231,12 +250,12 @@ template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
 };
 
 // ---- lists ------------------------------------------------------------------------------------------------------------------
-// Tokens sorted by slot (tokens without one last, in the group `slots`), in the order of the batch inside a slot; tiles of up to
-// 128 tokens of one slot.  One CTA: every warp counts a run of tokens, then places it.
+// Tokens sorted by slot (tokens without one last, in the group `slots`), in the order of the batch inside a slot, every slot's from a
+// multiple of sixteen on; tiles of up to 128 tokens of one slot.  One CTA: every warp counts a run of tokens, then places it.
 struct ATile { uint32_t slot, first, rows, pad; };
 
 __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__restrict__ ids, uint32_t T, uint32_t S, uint32_t *__restrict__ order,
-                                                             uint32_t *__restrict__ offsets, ATile *__restrict__ tiles, uint32_t *__restrict__ n_tiles,
+                                                             uint32_t *__restrict__ offsets /* [groups][start, tokens] */, ATile *__restrict__ tiles, uint32_t *__restrict__ n_tiles,
                                                              uint32_t *status) {
     extern __shared__ uint32_t counts[];                     // [warps][S + 1], then the groups' tokens [S + 1]
     __shared__ uint32_t sums[2][32];
@@ -281,7 +300,8 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
     // where each group and its tiles start: two groups to a thread
     uint32_t total[2], rows_before = 0, tiles_before = 0;
     for (uint32_t j = 0; j < 2; j++) total[j] = 2 * threadIdx.x + j < G ? totals[2 * threadIdx.x + j] : 0;
-    uint32_t r = total[0] + total[1], n = (total[0] + TM - 1) / TM + (total[1] + TM - 1) / TM;
+    const uint32_t room[2] = {(total[0] + 15) & ~15u, (total[1] + 15) & ~15u};
+    uint32_t r = room[0] + room[1], n = (total[0] + TM - 1) / TM + (total[1] + TM - 1) / TM;
     const uint32_t own_r = r, own_n = n;
     for (uint32_t o = 1; o < 32; o <<= 1) {
         const uint32_t a = __shfl_up_sync(0xffffffffu, r, o), b = __shfl_up_sync(0xffffffffu, n, o);
@@ -296,10 +316,11 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
         const uint32_t g = 2 * threadIdx.x + j;
         if (g >= G) break;
         totals[g] = rows_before;
-        offsets[g] = rows_before;
+        offsets[2 * g] = rows_before;
+        offsets[2 * g + 1] = total[j];
         for (uint32_t at = 0; at < total[j]; at += TM) tiles[tiles_before++] = ATile{g, rows_before + at, min(TM, total[j] - at), 0};
-        rows_before += total[j];
-        if (g == S) { offsets[G] = rows_before; *n_tiles = tiles_before; }
+        rows_before += room[j];
+        if (g == S) *n_tiles = tiles_before;
     }
     __syncthreads();
     if (per > 32 * AHEAD) fetch(first);                      // else they are still there
@@ -361,14 +382,14 @@ __device__ __forceinline__ void step_mma(uint32_t d, uint32_t d_step, uint32_t s
         tc_mma(d + k % MAINS * d_step, a + (k * TA::k16(AMN) >> 4), b + (k * TB::k16(BMN) >> 4), idesc, d_step == 0 || k >= MAINS ? 1 : more);
 }
 // Sixteen columns of a sum that lies in the accumulators of shrink and outer.
-template <uint32_t RP> __device__ __forceinline__ void load_sum(uint32_t addr, float (&v)[16]) {
+template <uint32_t RP> __device__ __forceinline__ void load_sum(uint32_t addr, float (&v)[16], uint32_t mains = Sums<RP>::MAINS) {
     float u[16];
     tc_load16(addr, v);
 #pragma unroll
     for (uint32_t m = 1; m <= Sums<RP>::MAINS; m++) {
         tc_load16(addr + m * RP, u);
 #pragma unroll
-        for (int i = 0; i < 16; i++) v[i] += u[i];
+        for (int i = 0; i < 16; i++) v[i] += m == Sums<RP>::MAINS || m < mains ? u[i] : 0.0f;
     }
 }
 
@@ -380,7 +401,7 @@ template <typename W> struct ShrinkJob {
     const float *x;
     uint64_t pitch;
     bool x_fours;                                            // rows on boundaries of four values, no more than 2^32 such runs
-    __nv_bfloat16 *planes;                                   // [3][rows][RP]: the result cut in three, rows in the lists' order
+    __nv_bfloat16 *planes;                                   // [3][rows x RP]: the result, rows in the lists' order
 };
 template <typename W> struct ShrinkArgs {
     ShrinkJob<W> job[2];
@@ -484,20 +505,23 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
     tc_after();
     if (warp == 0) tc_free(tmem, Sums<RP>::COLS);
     const float scale = a.scale ? a.scale[t.slot] : 1.0f;
-    const uint32_t rows = TM / parts;
+    const uint32_t rows = TM / parts, rows16 = (t.rows + 15) & ~15u;
     for (uint32_t u = tid; u < rows * (RP / 4); u += THREADS) {
-        const uint32_t row = part * rows + u / (RP / 4), c = u % (RP / 4) * 4;
-        if (row >= t.rows) break;
-        float4 sum = make_float4(0, 0, 0, 0);
-        for (uint32_t p = 0; p < parts; p++) {
-            const float4 v = *(const float4 *)(cluster.map_shared_rank(acc, p) + row * M::PITCH + c);
-            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-        }
-        sum.x *= scale; sum.y *= scale; sum.z *= scale; sum.w *= scale;
+        // two threads to eight values of a row, eight rows to 128 bytes of the result
+        const uint32_t row = part * rows + u / (2 * RP) * 8 + (u >> 1 & 7), c = (u >> 4) % (RP / 8) * 8 + (u & 1) * 4;
+        if (row >= rows16) break;
+        float4 v[8], sum = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (uint32_t p = 0; p < 8; p++) if (p < parts) v[p] = *(const float4 *)(cluster.map_shared_rank(acc, p) + row * M::PITCH + c);
+#pragma unroll
+        for (uint32_t p = 0; p < 8; p++) if (p < parts) { sum.x += v[p].x; sum.y += v[p].y; sum.z += v[p].z; sum.w += v[p].w; }
+        const bool there = row < t.rows;
+        sum = make_float4(there ? sum.x * scale : 0, there ? sum.y * scale : 0, there ? sum.z * scale : 0, there ? sum.w * scale : 0);
+        __nv_bfloat16 *to = job.planes + (uint64_t)((t.first + row) >> 3) * (8 * RP) + (c >> 3) * 64 + (row & 7) * 8 + (c & 7);
 #pragma unroll
         for (int p = 0; p < 3; p++) {
             const uint32_t lo = cut2(sum.x, sum.y), hi = cut2(sum.z, sum.w);
-            *(uint2 *)(job.planes + p * a.plane + (uint64_t)(t.first + row) * RP + c) = make_uint2(lo, hi);
+            *(uint2 *)(to + p * a.plane) = make_uint2(lo, hi);
         }
     }
     cluster.sync();                                          // nobody leaves while its sums are read
@@ -506,7 +530,7 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
 // ---- expand -----------------------------------------------------------------------------------------------------------------
 template <typename W> struct ExpandArgs {
     Mat<W> w;
-    const __nv_bfloat16 *planes;                             // [3][rows][RP], of shrink
+    const __nv_bfloat16 *planes;                             // of shrink
     uint64_t plane;
     Lists lists;
     uint32_t slots, blocks;                                  // blocks of 128 columns per CTA
@@ -517,7 +541,7 @@ template <typename W> struct ExpandArgs {
     uint32_t *status;
 };
 template <typename W, uint32_t RP> struct ExpandMap {
-    using H = Tile<TM, RP, 3>;                               // rows tokens: K-major
+    using H = Rank<TM, RP>;                                  // rows tokens: K-major
     using Run = MatRun<W, RP, 128>;                          // Tall: K-major, Wide: MN-major
     static constexpr uint32_t PLACES = 64, H_AT = PLACES + TM * 16, W_AT = H_AT + H::BYTES, NEED = W_AT + Run::BYTES;
     // Never more than four CTAs on an SM, which have its 512 columns of TMEM: a fifth would hold its place waiting for columns (233472
@@ -525,9 +549,6 @@ template <typename W, uint32_t RP> struct ExpandMap {
     static constexpr uint32_t TOTAL = NEED < 46080 ? 46080 : NEED, CTAS = TOTAL < 75000 ? 3 : TOTAL < 115000 ? 2 : 1;
     static_assert(5 * (TOTAL + 1024) > 233472 && TM == 128, "at most four CTAs of 128 TMEM columns");
 };
-
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Columns of the projection are the accumulator's lanes and tokens its columns, so that a warp's 32 lanes hold 32 neighbouring values
 // of a token's row.  base is read a batch of sixteen rows ahead of the one that is added.
@@ -546,7 +567,7 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
     if (none && a.base == a.y) return;
     const Mat<W> m = a.w;
     const uint32_t first = blockIdx.x * a.blocks, last = min((m.width + 127) / 128, first + a.blocks);
-    if (tid == 0) bar_init(base);
+    if (tid < 2) bar_init(base + 8 * tid);                   // products, rows of shrink
     if (warp == 0) tc_alloc(base + 32, TM);
     if (tid < TM) {
         const uint64_t row = a.lists.order[t.first + min(tid, t.rows - 1)];
@@ -556,17 +577,13 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
     typename M::Run wv;
     const uint32_t n = uniform((t.rows + 15) & ~15u);
     if (!none) {
-        for (uint32_t u = tid; u < 3 * t.rows * (RP / 8); u += THREADS) {
-            const uint32_t p = u / (t.rows * (RP / 8)), v = u % (t.rows * (RP / 8)), row = v / (RP / 8), c = v % (RP / 8) * 8;
-            copy16(base + M::H_AT + p * M::H::PLANE + M::H::at(row, c), a.planes + p * a.plane + (uint64_t)(t.first + row) * RP + c);
-        }
         wv.begin(m, first * 128);
         wv.load(m, w, first * 128, m.width);
-        copies_done();
     }
     tc_before();
     __syncthreads();
     tc_after();
+    if (tid == 0 && !none) copy_rank<TM, RP>(base + M::H_AT, a.planes, a.plane, t.first, n, base + 8);
     const uint32_t tmem = uniform(*(volatile uint32_t *)(smem + 32));
     const uint32_t idesc = idesc_of(128, n, m.wide, false);
     const uint32_t t_first = (warp >> 2) * 64, t_last = min(t.rows, t_first + 64), d = tmem + ((warp & 3) << 21);
@@ -589,6 +606,8 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
             __syncthreads();
             if (warp == 0) {
                 tc_after();
+                if (block == first) bar_wait(base + 8, 0, a.status);
+                __syncwarp();
                 const uint32_t leader = elect();
                 if (m.wide) step_mma<typename M::Run::Wide, typename M::H, M::Run::PLANES, 3, true, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
                 else step_mma<typename M::Run::Tall, typename M::H, M::Run::PLANES, 3, false, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
@@ -622,7 +641,7 @@ struct OuterJob {
     uint64_t pitch;
     uint32_t width;
     bool x_fours;
-    const __nv_bfloat16 *planes;                             // [3][rows][RP]
+    const __nv_bfloat16 *planes;                             // of shrink
     float *d;                                                // [slots][rank * width]: (r, c) at r * sr + c * sc
     uint32_t sr, sc;
     uint32_t blocks;                                         // of 128 columns
@@ -636,9 +655,9 @@ struct OuterArgs {
 };
 template <uint32_t RP> struct OuterMap {
     using X = Tile<TC, 128, 3>;                              // rows tokens: MN-major
-    using H = Tile<TC, RP, 3>;                               // rows tokens: MN-major
+    using H = Rank<TC, RP>;                                  // rows tokens: MN-major
     static constexpr uint32_t STAGE = 64, H_AT = STAGE + X::BYTES, END = H_AT + H::BYTES;
-    static constexpr uint32_t PITCH = 129;                   // floats per r of the exchanged accumulators
+    static constexpr uint32_t PITCH = 132;                   // floats per r of the exchanged accumulators
     static constexpr uint32_t ACC_END = STAGE + RP * PITCH * 4, TOTAL = END > ACC_END ? END : ACC_END;
 };
 
@@ -655,14 +674,14 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     const uint32_t c0 = (blockIdx.y - (second ? a.job[0].blocks : 0)) * 128;
     grid_wait();
     grid_go();
-    const uint32_t begin = a.lists.offsets[slot], tokens = a.lists.offsets[slot + 1] - begin;
+    const uint32_t begin = a.lists.offsets[2 * slot], tokens = a.lists.offsets[2 * slot + 1];
     const uint32_t cols = min(128u, job.width - c0), sr = job.sr, sc = job.sc;
     float *d = job.d + (uint64_t)slot * a.rank * job.width + c0 * sc;
     if (!tokens) {
         for (uint32_t u = part * THREADS + tid; u < a.rank * cols; u += parts * THREADS) d[sc == 1 ? u / cols * sr + u % cols : u % a.rank * sr + u / a.rank * sc] = 0;
         return;                                              // the same for all CTAs of the cluster
     }
-    if (tid == 0) bar_init(base);
+    if (tid < 2) bar_init(base + 8 * tid);                   // products, rows of shrink
     if (warp == 0) tc_alloc(base + 32, Sums<RP>::COLS);
     tc_before();
     __syncthreads();
@@ -670,7 +689,7 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     const uint32_t tmem = uniform(*(volatile uint32_t *)(smem + 32));
     const uint32_t per = ((tokens + parts - 1) / parts + TC - 1) / TC * TC, from = min(tokens, part * per), to = min(tokens, from + per);
     const uint32_t steps = uniform((to - from + TC - 1) / TC);
-    constexpr uint32_t XU = TC * 128 / 4 / THREADS, HU = TC * RP / 8;
+    constexpr uint32_t XU = TC * 128 / 4 / THREADS;
     const uint32_t x_row = tid / 32, x_col = lane * 4;
     const float *x = job.x + c0;
     Four<float> xv[XU];
@@ -694,21 +713,24 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     for (uint32_t s = 0; s < steps; s++) {
         const uint32_t t0 = from + s * TC;
         if (s) bar_wait(base, (s - 1) & 1, a.status);
-        for (uint32_t u = tid; u < 3 * HU; u += THREADS) {   // out of L2, under the cutting of x
-            const uint32_t p = u / HU, v = u % HU, row = v / (RP / 8), c = v % (RP / 8) * 8, to_at = base + M::H_AT + p * M::H::PLANE + M::H::at(row, c);
-            if (t0 + row < to) copy16(to_at, job.planes + p * a.plane + (uint64_t)(begin + t0 + row) * RP + c);
-            else put16(to_at, make_uint4(0, 0, 0, 0));       // a token that is not there adds nothing
-        }
+        const uint32_t rows16 = uniform((min(to - t0, TC) + 15) & ~15u);
+        if (tid == 0) copy_rank<TC, RP>(base + M::H_AT, job.planes, a.plane, begin + t0, rows16, base + 8);       // out of L2, while x is cut
 #pragma unroll
         for (uint32_t i = 0; i < XU; i++) xv[i].put(base + M::STAGE + M::X::at(x_row + i * 8, x_col), M::X::PLANE);
         if (s + 1 < steps) fetch(t0 + TC);
-        copies_done();
         fence_async();
         __syncthreads();
         if (warp == 0) {
             tc_after();
+            bar_wait(base + 8, s & 1, a.status);
+            __syncwarp();
             const uint32_t leader = elect();
-            step_mma<typename M::X, typename M::H, 3, 3, true, true, Sums<RP>::MAINS, TC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::H_AT, idesc, s == 0, leader);
+            if (rows16 == TC)
+                step_mma<typename M::X, typename M::H, 3, 3, true, true, Sums<RP>::MAINS, TC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::H_AT, idesc, s == 0, leader);
+            else                                             // the last tokens; into one of the leading accumulators alone, the others as they are
+                for (uint32_t k = 0; k < rows16 / 16; k++)
+                    step_mma<typename M::X, typename M::H, 3, 3, true, true, 1, 1>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE + k * M::X::k16(true),
+                                                                                    base + M::H_AT + k * M::H::k16(true), idesc, s == 0 && k == 0, leader);
             if (leader) tc_commit(base);
         }
     }
@@ -717,7 +739,7 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     float *acc = (float *)(smem + M::STAGE);
     for (uint32_t c = (warp >> 2) * 16; c < RP; c += 32) {
         float v[16];
-        load_sum<RP>(tmem + ((warp & 3) << 21) + c, v);
+        load_sum<RP>(tmem + ((warp & 3) << 21) + c, v, to - from + 15 < TC ? 1 : Sums<RP>::MAINS);
 #pragma unroll
         for (uint32_t i = 0; i < 16; i++) acc[(c + i) * M::PITCH + (warp & 3) * 32 + lane] = steps ? v[i] : 0.0f;
     }
@@ -725,11 +747,20 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     cluster.sync();
     tc_after();
     if (warp == 0) tc_free(tmem, Sums<RP>::COLS);
-    for (uint32_t u = part * THREADS + tid; u < a.rank * cols; u += parts * THREADS) {
-        const uint32_t r = sc == 1 ? u / cols : u % a.rank, c = sc == 1 ? u % cols : u / a.rank;
-        float sum = 0;
-        for (uint32_t p = 0; p < parts; p++) sum += cluster.map_shared_rank(acc, p)[r * M::PITCH + c];
-        d[r * sr + c * sc] = sum;
+    for (uint32_t u = part * THREADS + tid; u < RP * 32; u += parts * THREADS) {
+        // neighbouring threads: neighbouring columns of dA, neighbouring r of dB
+        const uint32_t r = sc == 1 ? u / 32 : u % RP, c = (sc == 1 ? u % 32 : u / RP) * 4;
+        if (r >= a.rank || c >= cols) continue;
+        float4 v[8], sum = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (uint32_t p = 0; p < 8; p++) if (p < parts) v[p] = *(const float4 *)(cluster.map_shared_rank(acc, p) + r * M::PITCH + c);
+#pragma unroll
+        for (uint32_t p = 0; p < 8; p++) if (p < parts) { sum.x += v[p].x; sum.y += v[p].y; sum.z += v[p].z; sum.w += v[p].w; }
+        float *to_at = d + r * sr + c * sc;
+        to_at[0] = sum.x;
+        if (c + 1 < cols) to_at[sc] = sum.y;
+        if (c + 2 < cols) to_at[2 * sc] = sum.z;
+        if (c + 3 < cols) to_at[3 * sc] = sum.w;
     }
     cluster.sync();
 }
@@ -765,7 +796,7 @@ int make_lists(const QW4ShTune *tune, const QW4CuAdapters *ad, const uint32_t *s
     s.T = (uint32_t)T; s.S = ad->slots; s.R = ad->rank; s.RP = qw4sh_adapter_rank(ad->rank);
     s.tiles = (uint32_t)qw4sh_adapter_tiles(T, s.S);
     s.lists = {tune->order, tune->offsets, (const ATile *)tune->tiles, tune->n_tiles};
-    s.scale = ad->scale; s.status = tune->status; s.plane = (uint64_t)T * s.RP; s.stream = stream;
+    s.scale = ad->scale; s.status = tune->status; s.plane = qw4sh_adapter_rows(T, s.S) * s.RP; s.stream = stream;
     return launch(adapter_lists_kernel, "adapter_lists_kernel", dim3(1), 1024, (size_t)33 * (s.S + 1) * 4, 0, false, stream, slots, s.T, s.S, tune->order,
                   tune->offsets, (ATile *)tune->tiles, tune->n_tiles, tune->status);
 }
@@ -799,7 +830,7 @@ template <uint32_t RP>
 int outer(const OuterJob *jobs, const Shape &s) {
     OuterArgs a = {{jobs[0], jobs[1]}, s.lists, s.plane, s.R, s.status};
     const uint32_t blocks = jobs[0].blocks + jobs[1].blocks;
-    const uint32_t c = cluster_of(blocks, s.T, TC);
+    const uint32_t c = cluster_of((uint64_t)blocks * ((s.T + 1023) / 1024 < s.S ? (s.T + 1023) / 1024 : s.S), s.T, TC);
     return launch(adapter_outer_kernel<RP>, "adapter_outer_kernel", dim3(c, blocks, s.S), THREADS, OuterMap<RP>::TOTAL, c, true, s.stream, a);
 }
 
@@ -834,6 +865,11 @@ int backward(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, Rows dy, Ro
 }  // namespace
 
 extern "C" uint32_t qw4sh_adapter_rank(uint32_t r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128; }
+// Places of the sorted tokens: every group rounded up to sixteen.
+extern "C" size_t qw4sh_adapter_rows(size_t tokens, uint32_t slots) {
+    const size_t groups = tokens < slots + 1u ? tokens : slots + 1u;
+    return (tokens + 15 * groups + 15) & ~(size_t)15;
+}
 // Most tiles that there can be: a token in each group, and then whole tiles.
 extern "C" size_t qw4sh_adapter_tiles(size_t tokens, uint32_t slots) {
     const size_t groups = tokens < slots + 1u ? tokens : slots + 1u;

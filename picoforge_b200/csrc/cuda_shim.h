@@ -246,12 +246,13 @@ typedef struct {
     unsigned long long *prob_sums;    /* [experts] units of 2^-40 */
     uint32_t *counts;             /* [experts + 1], and one ticket behind them */
     /* adapters: tokens sorted by slot, and tiles of them (16 bytes each) */
-    uint32_t *order, *offsets;    /* [tokens], [slots + 2] */
+    uint32_t *order, *offsets;    /* [qw4sh_adapter_rows(tokens, slots)], [slots + 1][start, tokens] */
     void *tiles;                  /* [qw4sh_adapter_tiles(tokens, slots)] */
     uint32_t *n_tiles;
     /* A x and B^T dy of every token, in that order, cut in three bf16 values */
-    void *h, *g;                  /* [3][tokens][qw4sh_adapter_rank(rank)] */
+    void *h, *g;                  /* [3][qw4sh_adapter_rows(tokens, slots) x qw4sh_adapter_rank(rank)] */
 } QW4ShTune;
+size_t qw4sh_adapter_rows(size_t tokens, uint32_t slots);
 size_t qw4sh_adapter_tiles(size_t tokens, uint32_t slots);
 uint32_t qw4sh_adapter_rank(uint32_t rank);
 int qw4sh_balance_forward(const QW4ShTune *tune, uint32_t experts, uint32_t k, const float *logits, size_t pitch, const uint32_t *ids,

@@ -61,9 +61,10 @@ Qwen4Status qw4cu_tune_work_create(const QW4CuTuneLimits *limits, QW4CuTuneWork 
     size_t at = 0;
     const size_t status = take(&at, 16), sums = take(&at, (size_t)l.experts * 8), counts = take(&at, ((size_t)l.experts + 2) * 4);
     const bool adapters = l.slots != 0;
-    const size_t order = take(&at, adapters ? l.tokens * 4 : 0), offsets = take(&at, adapters ? ((size_t)l.slots + 2) * 4 : 0);
+    const size_t places = adapters ? qw4sh_adapter_rows(l.tokens, l.slots) : 0;
+    const size_t order = take(&at, places * 4), offsets = take(&at, adapters ? ((size_t)l.slots + 1) * 8 : 0);
     const size_t tiles = take(&at, adapters ? qw4sh_adapter_tiles(l.tokens, l.slots) * 16 : 0), n_tiles = take(&at, 4);
-    const size_t rows = adapters ? 3 * l.tokens * qw4sh_adapter_rank(l.rank) * 2 : 0, h = take(&at, rows), g = take(&at, rows);
+    const size_t rows = adapters ? 3 * places * qw4sh_adapter_rank(l.rank) * 2 : 0, h = take(&at, rows), g = take(&at, rows);
     w->device_bytes = at;
     w->block = qw4sh_malloc(at);
     void *stream = NULL;

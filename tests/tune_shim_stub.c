@@ -9,6 +9,7 @@ int stub_device, stub_launches, stub_fail_launch, stub_fail_malloc;
 uint32_t stub_status[2] = {0, 0xffffffffu};             /* what the next sync finds */
 
 size_t qw4sh_adapter_tiles(size_t tokens, uint32_t slots) { return tokens + slots; }
+size_t qw4sh_adapter_rows(size_t tokens, uint32_t slots) { return tokens + slots; }
 uint32_t qw4sh_adapter_rank(uint32_t rank) { return rank; }
 int qw4sh_current_device(void) { return stub_device; }
 int qw4sh_device_count(void) { return 2; }
