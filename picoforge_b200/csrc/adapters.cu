@@ -255,32 +255,38 @@ template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
 struct ATile { uint32_t slot, first, rows, pad; };
 
 __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__restrict__ ids, uint32_t T, uint32_t S, uint32_t *__restrict__ order,
-                                                             uint32_t *__restrict__ offsets /* [groups][start, tokens] */, ATile *__restrict__ tiles, uint32_t *__restrict__ n_tiles,
-                                                             uint32_t *status) {
-    extern __shared__ uint32_t counts[];                     // [warps][S + 1], then the groups' tokens [S + 1]
+                                                             uint32_t *__restrict__ offsets /* [groups][start, tokens] */, ATile *__restrict__ tiles,
+                                                             uint32_t *__restrict__ n_tiles, uint32_t *status) {
+    extern __shared__ uint32_t counts[];                     // [warps][S + 1], then where the groups start [S + 1]
     __shared__ uint32_t sums[2][32];
     const uint32_t G = S + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t per = ((T + 31) / 32 + 31) & ~31u, first = min(T, warp * per), end = min(T, first + per);
-    uint32_t *mine = counts + warp * G, *totals = counts + 32 * G;
+    uint32_t *mine = counts + warp * G, *starts = counts + 32 * G;
     grid_go();                                               // the tiles' CTAs may take their places
     constexpr uint32_t AHEAD = 8;                            // loads in flight
-    uint32_t s[AHEAD];
+    uint32_t s[AHEAD], same[AHEAD];
     auto fetch = [&](uint32_t t0) {
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; i++) s[i] = ids[min(t0 + 32 * i + lane, T - 1)];
+        for (uint32_t i = 0; i < AHEAD; i++) s[i] = t0 + 32 * i + lane < end ? ids[t0 + 32 * i + lane] : 0;
+    };
+    auto match = [&](uint32_t t0) {
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; i++) {
+            const bool there = t0 + 32 * i + lane < end;
+            if (there && s[i] >= S && s[i] != QW4CU_NO_ADAPTER) atomicOr(status, QW4SH_ERR_BOUNDS);
+            s[i] = there ? min(s[i], S) : 0xffffffffu;
+            same[i] = t0 + 32 * i < end ? __match_any_sync(0xffffffffu, s[i]) : 0;
+        }
     };
     fetch(first);
     for (uint32_t i = threadIdx.x; i < 32 * G; i += 1024) counts[i] = 0;
+    match(first);
     __syncthreads();
     for (uint32_t t0 = first; t0 < end; t0 += 32 * AHEAD) {
-        if (t0 != first) fetch(t0);
+        if (t0 != first) { fetch(t0); match(t0); }
 #pragma unroll
         for (uint32_t i = 0; i < AHEAD; i++) {
-            if (t0 + 32 * i >= end) break;
-            const bool there = t0 + 32 * i + lane < end;
-            if (there && s[i] >= S && s[i] != QW4CU_NO_ADAPTER) atomicOr(status, QW4SH_ERR_BOUNDS);
-            const uint32_t g = there ? min(s[i], S) : 0xffffffffu, same = __match_any_sync(0xffffffffu, g);
-            if (there && __ffs(same) - 1 == (int)lane) mine[g] += __popc(same);
+            if (s[i] <= S && __ffs(same[i]) - 1 == (int)lane) mine[s[i]] += __popc(same[i]);
             __syncwarp();
         }
     }
@@ -294,13 +300,15 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
             if (lane >= o) sum += u;
         }
         counts[lane * G + g] = sum - c;
-        if (lane == 31) totals[g] = sum;
+        if (lane == 31) starts[g] = sum;
     }
     __syncthreads();
     // where each group and its tiles start: two groups to a thread
-    uint32_t total[2], rows_before = 0, tiles_before = 0;
-    for (uint32_t j = 0; j < 2; j++) total[j] = 2 * threadIdx.x + j < G ? totals[2 * threadIdx.x + j] : 0;
-    const uint32_t room[2] = {(total[0] + 15) & ~15u, (total[1] + 15) & ~15u};
+    uint32_t total[2], room[2];
+    for (uint32_t j = 0; j < 2; j++) {
+        total[j] = 2 * threadIdx.x + j < G ? starts[2 * threadIdx.x + j] : 0;
+        room[j] = (total[j] + 15) & ~15u;
+    }
     uint32_t r = room[0] + room[1], n = (total[0] + TM - 1) / TM + (total[1] + TM - 1) / TM;
     const uint32_t own_r = r, own_n = n;
     for (uint32_t o = 1; o < 32; o <<= 1) {
@@ -309,33 +317,30 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
     }
     if (lane == 31) { sums[0][warp] = r; sums[1][warp] = n; }
     __syncthreads();
-    for (uint32_t w = 0; w < warp; w++) { rows_before += sums[0][w]; tiles_before += sums[1][w]; }
-    rows_before += r - own_r;
-    tiles_before += n - own_n;
+    uint32_t at = __reduce_add_sync(0xffffffffu, lane < warp ? sums[0][lane] : 0) + r - own_r;
+    uint32_t tile = __reduce_add_sync(0xffffffffu, lane < warp ? sums[1][lane] : 0) + n - own_n;
     for (uint32_t j = 0; j < 2; j++) {
         const uint32_t g = 2 * threadIdx.x + j;
         if (g >= G) break;
-        totals[g] = rows_before;
-        offsets[2 * g] = rows_before;
+        starts[g] = at;
+        offsets[2 * g] = at;
         offsets[2 * g + 1] = total[j];
-        for (uint32_t at = 0; at < total[j]; at += TM) tiles[tiles_before++] = ATile{g, rows_before + at, min(TM, total[j] - at), 0};
-        rows_before += room[j];
-        if (g == S) *n_tiles = tiles_before;
+        for (uint32_t i = 0; i < total[j]; i += TM) tiles[tile++] = ATile{g, at + i, min(TM, total[j] - i), 0};
+        at += room[j];
+        if (g == S) *n_tiles = tile;
     }
     __syncthreads();
-    if (per > 32 * AHEAD) fetch(first);                      // else they are still there
+    if (per > 32 * AHEAD) { fetch(first); match(first); }    // else they are still there
     for (uint32_t t0 = first; t0 < end; t0 += 32 * AHEAD) {
-        if (t0 != first) fetch(t0);
+        if (t0 != first) { fetch(t0); match(t0); }
 #pragma unroll
         for (uint32_t i = 0; i < AHEAD; i++) {
-            if (t0 + 32 * i >= end) break;
-            const bool there = t0 + 32 * i + lane < end;
-            const uint32_t g = there ? min(s[i], S) : 0xffffffffu, same = __match_any_sync(0xffffffffu, g);
-            const uint32_t at = there ? mine[g] : 0;
+            const bool there = s[i] <= S;
+            const uint32_t before = there ? mine[s[i]] : 0;
             __syncwarp();
             if (there) {
-                order[totals[g] + at + __popc(same & ((1u << lane) - 1))] = t0 + 32 * i + lane;
-                if (__ffs(same) - 1 == (int)lane) mine[g] = at + __popc(same);
+                order[starts[s[i]] + before + __popc(same[i] & ((1u << lane) - 1))] = t0 + 32 * i + lane;
+                if (__ffs(same[i]) - 1 == (int)lane) mine[s[i]] = before + __popc(same[i]);
             }
             __syncwarp();
         }
@@ -478,7 +483,6 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
 #pragma unroll
         for (uint32_t i = 0; i < XU; i++) xv[i].put(base + M::STAGE + M::X::at(x_row + i * ROWS, x_col), M::X::PLANE);
         wv.put(m, c0, c_end, base + M::W_AT);
-        if (s + 1 < steps) fetch(c0 + KC);
         fence_async();
         __syncthreads();
         if (warp == 0) {
@@ -487,7 +491,9 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
             if (m.wide) step_mma<typename M::X, typename M::Run::Wide, 3, M::Run::PLANES, false, false, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::W_AT, idesc, s == 0, leader);
             else step_mma<typename M::X, typename M::Run::Tall, 3, M::Run::PLANES, false, true, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::W_AT, idesc, s == 0, leader);
             if (leader) tc_commit(base);
+            __syncwarp();
         }
+        if (s + 1 < steps) fetch(c0 + KC);                   // behind the products: the SM takes no more loads than it has lines for, and makes them wait
     }
     if (steps) bar_wait(base, (steps - 1) & 1, a.status);
     tc_after();
@@ -597,10 +603,9 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
 #pragma unroll
             for (uint32_t i = 0; i < 16; i++) b[i] = *(const float *)(b_col + place[j + i].b);
         };
-        if (added && t_first < t_last) fetch(t_first);
+        if (none && added && t_first < t_last) fetch(t_first);
         if (!none) {
             wv.put(m, block * 128, m.width, base + M::W_AT);
-            if (block + 1 < last) wv.load(m, w, (block + 1) * 128, m.width);
             fence_async();
             tc_before();
             __syncthreads();
@@ -612,7 +617,10 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
                 if (m.wide) step_mma<typename M::Run::Wide, typename M::H, M::Run::PLANES, 3, true, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
                 else step_mma<typename M::Run::Tall, typename M::H, M::Run::PLANES, 3, false, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
                 if (leader) tc_commit(base);
+                __syncwarp();
             }
+            if (added && t_first < t_last) fetch(t_first);
+            if (block + 1 < last) wv.load(m, w, (block + 1) * 128, m.width);
             bar_wait(base, (block - first) & 1, a.status);
             tc_after();
         }
@@ -717,7 +725,6 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
         if (tid == 0) copy_rank<TC, RP>(base + M::H_AT, job.planes, a.plane, begin + t0, rows16, base + 8);       // out of L2, while x is cut
 #pragma unroll
         for (uint32_t i = 0; i < XU; i++) xv[i].put(base + M::STAGE + M::X::at(x_row + i * 8, x_col), M::X::PLANE);
-        if (s + 1 < steps) fetch(t0 + TC);
         fence_async();
         __syncthreads();
         if (warp == 0) {
@@ -732,7 +739,9 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
                     step_mma<typename M::X, typename M::H, 3, 3, true, true, 1, 1>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE + k * M::X::k16(true),
                                                                                     base + M::H_AT + k * M::H::k16(true), idesc, s == 0 && k == 0, leader);
             if (leader) tc_commit(base);
+            __syncwarp();
         }
+        if (s + 1 < steps) fetch(t0 + TC);
     }
     if (steps) bar_wait(base, (steps - 1) & 1, a.status);
     tc_after();
