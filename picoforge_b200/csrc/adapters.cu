@@ -774,6 +774,154 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     cluster.sync();
 }
 
+// ---- a few tokens -----------------------------------------------------------------------------------------------------------
+// One cluster of eight CTAs to a token, whatever its slot: A x with a run of columns of x to each CTA, the eight partial sums of every r
+// to all of them (distributed shared memory), B h with a run of y's columns to each.  Everything is read once and one launch is all
+// there is.  What bounds it is latency: the id, then A, the exchange, then the sum; B and base are on their way meanwhile.
+constexpr uint32_t FEW_CTAS = 8, FEW_TOKENS = 128;
+
+template <typename W> struct FewArgs {
+    const W *a, *b;
+    uint32_t slots, rank, k, n;
+    const float *scale, *x;
+    uint64_t x_pitch;
+    const uint32_t *ids;
+    const float *base;
+    uint64_t base_pitch;
+    float *y;
+    uint64_t y_pitch;
+    bool x_fours;
+    uint32_t *status;
+};
+
+// V neighbouring values of a row in one load, and their products with floats.
+template <typename W, int V> struct Run;
+template <int V> struct Run<float, V> {
+    float v[V];
+    __device__ __forceinline__ void load(const float *p) {
+        if (V == 4) { const float4 u = *(const float4 *)p; v[0] = u.x; v[V / 4] = u.y; v[V / 2] = u.z; v[V - 1] = u.w; }
+        else v[0] = *p;
+    }
+    __device__ __forceinline__ float dot(const float *f, float sum) const {
+#pragma unroll
+        for (int i = 0; i < V; i++) sum = fmaf(v[i], f[i], sum);
+        return sum;
+    }
+};
+__device__ __forceinline__ float2 pair_of(uint32_t u, const __nv_bfloat16 *) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+__device__ __forceinline__ float2 pair_of(uint32_t u, const __half *) { return __half22float2(*(const __half2 *)&u); }
+template <typename H, int V> struct Run16 {
+    uint32_t v[V > 1 ? V / 2 : 1];
+    __device__ __forceinline__ void load(const H *p) {
+        if (V == 8) { const uint4 u = *(const uint4 *)p; v[0] = u.x; v[V / 8] = u.y; v[V / 4] = u.z; v[V / 2 - 1] = u.w; }
+        else if (V == 4) { const uint2 u = *(const uint2 *)p; v[0] = u.x; v[V / 4] = u.y; }
+        else v[0] = *(const uint16_t *)p;
+    }
+    __device__ __forceinline__ float dot(const float *f, float sum) const {
+        if (V == 1) return fmaf(pair_of(v[0], (const H *)nullptr).x, f[0], sum);
+#pragma unroll
+        for (int i = 0; i < V / 2; i++) {
+            const float2 u = pair_of(v[i], (const H *)nullptr);
+            sum = fmaf(u.y, f[2 * i + 1], fmaf(u.x, f[2 * i], sum));
+        }
+        return sum;
+    }
+};
+template <int V> struct Run<__nv_bfloat16, V> : Run16<__nv_bfloat16, V> {};
+template <int V> struct Run<__half, V> : Run16<__half, V> {};
+
+template <typename W, int V>
+__global__ void __launch_bounds__(THREADS) adapter_few_kernel(const __grid_constant__ FewArgs<W> a) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    __shared__ float partial[FEW_CTAS][QW4CU_TUNE_MAX_RANK], h[QW4CU_TUNE_MAX_RANK];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, part = blockIdx.x, t = blockIdx.y, R = a.rank;
+    const uint32_t s = a.ids[t];
+    const uint32_t n_per = (a.n + FEW_CTAS - 1) / FEW_CTAS, n0 = min(a.n, part * n_per), n1 = min(a.n, n0 + n_per);
+    const float *base = a.base ? a.base + t * a.base_pitch : nullptr;
+    float *y = a.y + t * a.y_pitch;
+    if (s >= a.slots) {                                      // the same for all CTAs of the cluster
+        if (s != QW4CU_NO_ADAPTER && tid == 0) atomicOr(a.status, QW4SH_ERR_BOUNDS);
+        if (base != y) for (uint32_t c = n0 + tid; c < n1; c += THREADS) y[c] = base ? base[c] : 0.0f;
+        return;
+    }
+    const W *A = a.a + (uint64_t)s * R * a.k, *B = a.b + (uint64_t)s * R * a.n;
+    const float *x = a.x + t * a.x_pitch;
+
+    // rows of B: `span` lanes to a row, so that a load of a warp is one run of memory
+    uint32_t span = 1;
+    while (span < 32 && span * V < R) span *= 2;
+    const uint32_t sub = lane % span, rows = 32 / span, n_first = n0 + warp * rows + lane / span, n_step = 8 * rows;
+    constexpr int PASSES = 4;
+    Run<W, V> bv[PASSES];
+    float added[PASSES];
+    auto fetch = [&](uint32_t n) {
+#pragma unroll
+        for (int i = 0; i < PASSES; i++) {
+            const uint32_t row = min(n + i * n_step, a.n - 1);
+            bv[i].load(B + (uint64_t)row * R + min(sub * V, R - V));
+            added[i] = base ? base[row] : 0.0f;
+        }
+    };
+    fetch(n_first);
+
+    const uint32_t k_per = ((a.k + V - 1) / V + FEW_CTAS - 1) / FEW_CTAS * V, c0 = min(a.k, part * k_per), c1 = min(a.k, c0 + k_per);
+    constexpr uint32_t RANKS = 4;                            // of a warp at a time
+    for (uint32_t r0 = warp; r0 < R; r0 += 8 * RANKS) {
+        float sum[RANKS] = {};
+        for (uint32_t c = c0 + lane * V; c < c1; c += 32 * V) {
+            float xv[V];
+            Run<W, V> av[RANKS];
+#pragma unroll
+            for (uint32_t j = 0; j < RANKS; j++) av[j].load(A + (uint64_t)min(r0 + 8 * j, R - 1) * a.k + c);
+            if (V >= 4 && a.x_fours) {
+#pragma unroll
+                for (int i = 0; i < V; i += 4) { const float4 u = *(const float4 *)(x + c + i); xv[i] = u.x; xv[(i + 1) % V] = u.y; xv[(i + 2) % V] = u.z; xv[(i + 3) % V] = u.w; }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) xv[i] = x[c + i];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < RANKS; j++) sum[j] = av[j].dot(xv, sum[j]);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < RANKS; j++)
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
+        if (lane < FEW_CTAS) {
+            float *to = cluster.map_shared_rank(&partial[part][0], lane);
+#pragma unroll
+            for (uint32_t j = 0; j < RANKS; j++) if (r0 + 8 * j < R) to[r0 + 8 * j] = sum[j];
+        }
+    }
+    cluster.sync();
+    if (tid < R) {
+        float sum = 0;
+#pragma unroll
+        for (uint32_t p = 0; p < FEW_CTAS; p++) sum += partial[p][tid];
+        h[tid] = sum * (a.scale ? a.scale[s] : 1.0f);
+    }
+    __syncthreads();
+    for (uint32_t n = n_first; n - lane / span < n1; n += PASSES * n_step) {
+        if (n != n_first) fetch(n);
+        float sum[PASSES];
+#pragma unroll
+        for (int i = 0; i < PASSES; i++) {
+            sum[i] = sub * V < R ? bv[i].dot(h + sub * V, 0.0f) : 0.0f;
+            for (uint32_t r = (sub + span) * V; r < R; r += span * V) {              // more values to a row than a warp has lanes for
+                Run<W, V> more;
+                more.load(B + (uint64_t)min(n + i * n_step, a.n - 1) * R + r);
+                sum[i] = more.dot(h + r, sum[i]);
+            }
+        }
+        for (uint32_t o = span / 2; o; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < PASSES; i++) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+#pragma unroll
+        for (int i = 0; i < PASSES; i++) if (sub == 0 && n + i * n_step < n1) y[n + i * n_step] = added[i] + sum[i];
+    }
+}
+
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 template <typename... A>
 int launch(void (*kernel)(A...), const char *name, dim3 grid, uint32_t threads, size_t smem, uint32_t cluster, bool behind, cudaStream_t stream, A... args) {
@@ -849,6 +997,15 @@ template <typename W> Mat<W> mat_b(const QW4CuAdapters *ad) { return {(const W *
 struct Rows { const float *p; size_t pitch; };
 bool runs(Rows x, uint64_t T) { return fours(x.p, x.pitch, 4) && T * x.pitch < 1ull << 34; }
 
+template <typename W>
+int few(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, const uint32_t *slots, Rows base, float *y, size_t y_pitch, size_t T, cudaStream_t stream) {
+    const FewArgs<W> a = {(const W *)ad->a, (const W *)ad->b, ad->slots, ad->rank, (uint32_t)ad->k, (uint32_t)ad->n, ad->scale, x.p, x.pitch, slots,
+                          base.p, base.pitch, y, y_pitch, fours(x.p, x.pitch, 4), tune->status};
+    constexpr int MOST = 16 / sizeof(W);
+    auto runs_of = [&](uint32_t v) { return ad->k % v == 0 && ad->rank % v == 0 && (((uintptr_t)ad->a | (uintptr_t)ad->b) & (v * sizeof(W) - 1)) == 0; };
+    const auto kernel = runs_of(MOST) ? adapter_few_kernel<W, MOST> : runs_of(4) ? adapter_few_kernel<W, 4> : adapter_few_kernel<W, 1>;
+    return launch(kernel, "adapter_few_kernel", dim3(FEW_CTAS, (unsigned)T), THREADS, 0, FEW_CTAS, false, stream, a);
+}
 template <typename W, uint32_t RP>
 int forward(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, Rows base, float *y, size_t y_pitch, const Shape &s) {
     const ShrinkJob<W> job = {mat_a<W>(ad), x.p, x.pitch, runs(x, s.T), (__nv_bfloat16 *)tune->h};
@@ -887,9 +1044,11 @@ extern "C" size_t qw4sh_adapter_tiles(size_t tokens, uint32_t slots) {
 
 extern "C" int qw4sh_adapter_forward(const QW4ShTune *tune, const QW4CuAdapters *ad, const float *x, size_t x_pitch, const uint32_t *slots,
                                      const float *base, size_t base_pitch, float *y, size_t y_pitch, size_t tokens, void *stream) {
+    const Rows xr = {x, x_pitch}, br = {base, base_pitch};
+    if (tokens <= FEW_TOKENS)
+        return (ad->type == 0 ? few<float> : ad->type == 1 ? few<__half> : few<__nv_bfloat16>)(tune, ad, xr, slots, br, y, y_pitch, tokens, (cudaStream_t)stream);
     Shape s;
     if (const int rc = make_lists(tune, ad, slots, tokens, (cudaStream_t)stream, s)) return rc;
-    const Rows xr = {x, x_pitch}, br = {base, base_pitch};
     return BY_TYPE(forward, tune, ad, xr, br, y, y_pitch, s);
 }
 
