@@ -831,7 +831,7 @@ template <int V> struct Run<__nv_bfloat16, V> : Run16<__nv_bfloat16, V> {};
 template <int V> struct Run<__half, V> : Run16<__half, V> {};
 
 template <typename W, int V>
-__global__ void __launch_bounds__(THREADS) adapter_few_kernel(const __grid_constant__ FewArgs<W> a) {
+__global__ void __launch_bounds__(THREADS, 4) adapter_few_kernel(const __grid_constant__ FewArgs<W> a) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ float partial[FEW_CTAS][QW4CU_TUNE_MAX_RANK], h[QW4CU_TUNE_MAX_RANK];
