@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
     const uint32_t per = ((T + 31) / 32 + 31) & ~31u, first = min(T, warp * per), end = min(T, first + per);
     uint32_t *mine = counts + warp * G, *starts = counts + 32 * G;
     grid_go();                                               // the tiles' CTAs may take their places
+    grid_wait();
     constexpr uint32_t AHEAD = 8;                            // loads in flight
     uint32_t s[AHEAD], same[AHEAD];
     auto fetch = [&](uint32_t t0) {
@@ -437,7 +438,6 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
     cg::cluster_group cluster = cg::this_cluster();          // the CTAs of one tile, a run of columns each
     const uint32_t parts = cluster.num_blocks(), part = cluster.block_rank();
     grid_wait();
-    grid_go();
     if (blockIdx.y >= *a.lists.n_tiles) return;              // the same for all CTAs of a cluster
     const ATile t = a.lists.tiles[blockIdx.y];
     if (t.slot >= a.slots) return;
@@ -497,6 +497,7 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
     }
     if (steps) bar_wait(base, (steps - 1) & 1, a.status);
     tc_after();
+    grid_go();                                               // not before: CTAs of the next launch would crowd onto the SMs that are done first
     // accumulators to shared memory, summed over the cluster's CTAs in their order, scaled, cut and stored
     float *acc = (float *)(smem + M::STAGE);
     for (uint32_t c = (warp >> 2) * 16; c < RP; c += 32) {
@@ -565,16 +566,15 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, base = smem_u32(smem);
     struct Place { uint64_t b, y; };                         // bytes from the first row of base and of y
     Place *place = (Place *)(smem + M::PLACES);
-    grid_wait();
     grid_go();
-    if (blockIdx.y >= *a.lists.n_tiles) return;
+    // The lists are there: the launch before this one, whose end grid_wait waits for, let this one start after its own wait for them.
+    if (blockIdx.y >= *a.lists.n_tiles) { grid_wait(); return; }                 // no launch ends before the one that it waits for
     const ATile t = a.lists.tiles[blockIdx.y];
     const bool none = t.slot >= a.slots;
-    if (none && a.base == a.y) return;
+    if (none && a.base == a.y) { grid_wait(); return; }
     const Mat<W> m = a.w;
     const uint32_t first = blockIdx.x * a.blocks, last = min((m.width + 127) / 128, first + a.blocks);
     if (tid < 2) bar_init(base + 8 * tid);                   // products, rows of shrink
-    if (warp == 0) tc_alloc(base + 32, TM);
     if (tid < TM) {
         const uint64_t row = a.lists.order[t.first + min(tid, t.rows - 1)];
         place[tid] = Place{row * a.base_pitch * 4, row * a.y_pitch * 4};
@@ -586,11 +586,15 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
         wv.begin(m, first * 128);
         wv.load(m, w, first * 128, m.width);
     }
+    if (warp == 0) tc_alloc(base + 32, TM);
     tc_before();
     __syncthreads();
     tc_after();
-    if (tid == 0 && !none) copy_rank<TM, RP>(base + M::H_AT, a.planes, a.plane, t.first, n, base + 8);
     const uint32_t tmem = uniform(*(volatile uint32_t *)(smem + 32));
+    if (tid == THREADS - 1) {
+        grid_wait();
+        if (!none) copy_rank<TM, RP>(base + M::H_AT, a.planes, a.plane, t.first, n, base + 8);
+    }
     const uint32_t idesc = idesc_of(128, n, m.wide, false);
     const uint32_t t_first = (warp >> 2) * 64, t_last = min(t.rows, t_first + 64), d = tmem + ((warp & 3) << 21);
     const bool added = a.base != nullptr;
@@ -603,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
 #pragma unroll
             for (uint32_t i = 0; i < 16; i++) b[i] = *(const float *)(b_col + place[j + i].b);
         };
-        if (none && added && t_first < t_last) fetch(t_first);
+        if (added && t_first < t_last && (none || block == first)) fetch(t_first);
         if (!none) {
             wv.put(m, block * 128, m.width, base + M::W_AT);
             fence_async();
@@ -619,7 +623,7 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
                 if (leader) tc_commit(base);
                 __syncwarp();
             }
-            if (added && t_first < t_last) fetch(t_first);
+            if (added && t_first < t_last && block != first) fetch(t_first);
             if (block + 1 < last) wv.load(m, w, (block + 1) * 128, m.width);
             bar_wait(base, (block - first) & 1, a.status);
             tc_after();
@@ -680,12 +684,12 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     const bool second = blockIdx.y >= a.job[0].blocks;
     const OuterJob &job = a.job[second];
     const uint32_t c0 = (blockIdx.y - (second ? a.job[0].blocks : 0)) * 128;
-    grid_wait();
-    grid_go();
+    // the lists are there, as for expand
     const uint32_t begin = a.lists.offsets[2 * slot], tokens = a.lists.offsets[2 * slot + 1];
     const uint32_t cols = min(128u, job.width - c0), sr = job.sr, sc = job.sc;
     float *d = job.d + (uint64_t)slot * a.rank * job.width + c0 * sc;
     if (!tokens) {
+        grid_wait();
         for (uint32_t u = part * THREADS + tid; u < a.rank * cols; u += parts * THREADS) d[sc == 1 ? u / cols * sr + u % cols : u % a.rank * sr + u / a.rank * sc] = 0;
         return;                                              // the same for all CTAs of the cluster
     }
@@ -717,6 +721,7 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
         if (t0 + TC < to) fetch_ids(t0 + TC);
     };
     if (steps) { fetch_ids(from); fetch(from); }
+    grid_wait();
     constexpr uint32_t idesc = idesc_of(128, RP, true, true);
     for (uint32_t s = 0; s < steps; s++) {
         const uint32_t t0 = from + s * TC;
@@ -745,6 +750,7 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     }
     if (steps) bar_wait(base, (steps - 1) & 1, a.status);
     tc_after();
+    grid_go();
     float *acc = (float *)(smem + M::STAGE);
     for (uint32_t c = (warp >> 2) * 16; c < RP; c += 32) {
         float v[16];
@@ -818,12 +824,13 @@ template <typename H, int V> struct Run16 {
         else v[0] = *(const uint16_t *)p;
     }
     __device__ __forceinline__ float dot(const float *f, float sum) const {
-        if (V == 1) return fmaf(pair_of(v[0], (const H *)nullptr).x, f[0], sum);
+        if constexpr (V == 1) sum = fmaf(pair_of(v[0], (const H *)nullptr).x, f[0], sum);
+        else
 #pragma unroll
-        for (int i = 0; i < V / 2; i++) {
-            const float2 u = pair_of(v[i], (const H *)nullptr);
-            sum = fmaf(u.y, f[2 * i + 1], fmaf(u.x, f[2 * i], sum));
-        }
+            for (int i = 0; i < V / 2; i++) {
+                const float2 u = pair_of(v[i], (const H *)nullptr);
+                sum = fmaf(u.y, f[2 * i + 1], fmaf(u.x, f[2 * i], sum));
+            }
         return sum;
     }
 };
@@ -836,6 +843,7 @@ __global__ void __launch_bounds__(THREADS, 4) adapter_few_kernel(const __grid_co
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ float partial[FEW_CTAS][QW4CU_TUNE_MAX_RANK], h[QW4CU_TUNE_MAX_RANK];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, part = blockIdx.x, t = blockIdx.y, R = a.rank;
+    grid_wait();
     const uint32_t s = a.ids[t];
     const uint32_t n_per = (a.n + FEW_CTAS - 1) / FEW_CTAS, n0 = min(a.n, part * n_per), n1 = min(a.n, n0 + n_per);
     const float *base = a.base ? a.base + t * a.base_pitch : nullptr;
@@ -954,14 +962,14 @@ int make_lists(const QW4ShTune *tune, const QW4CuAdapters *ad, const uint32_t *s
     s.tiles = (uint32_t)qw4sh_adapter_tiles(T, s.S);
     s.lists = {tune->order, tune->offsets, (const ATile *)tune->tiles, tune->n_tiles};
     s.scale = ad->scale; s.status = tune->status; s.plane = qw4sh_adapter_rows(T, s.S) * s.RP; s.stream = stream;
-    return launch(adapter_lists_kernel, "adapter_lists_kernel", dim3(1), 1024, (size_t)33 * (s.S + 1) * 4, 0, false, stream, slots, s.T, s.S, tune->order,
+    return launch(adapter_lists_kernel, "adapter_lists_kernel", dim3(1), 1024, (size_t)33 * (s.S + 1) * 4, 0, true, stream, slots, s.T, s.S, tune->order,
                   tune->offsets, (ATile *)tune->tiles, tune->n_tiles, tune->status);
 }
 
 // As many CTAs to a tile as give every SM two, a run of 128 columns each at least.
-uint32_t cluster_of(uint64_t items, uint64_t length, uint32_t least) {
+uint32_t cluster_of(uint64_t items, uint64_t length, uint32_t least, uint32_t most = 8) {
     uint32_t c = 1;
-    while (c < 8 && items * c < 2 * SMS && length / (2 * c) >= least) c *= 2;
+    while (c < most && items * c < 2 * SMS && length / (2 * c) >= least) c *= 2;
     return c;
 }
 
@@ -971,15 +979,14 @@ int shrink(const ShrinkJob<W> *jobs, uint32_t n, const Shape &s) {
     uint64_t width = 0;
     for (uint32_t i = 0; i < n; i++) { a.job[i] = jobs[i]; if (jobs[i].w.width > width) width = jobs[i].w.width; }
     a.lists = s.lists; a.scale = s.scale; a.plane = s.plane; a.slots = s.S; a.status = s.status;
-    const uint32_t c = cluster_of((uint64_t)(s.T + TM - 1) / TM * n, width, 128);
+    const uint32_t c = cluster_of((uint64_t)(s.T + TM - 1) / TM * n, width, 128, s.T > 4096 ? 4 : 8);
     return launch(adapter_shrink_kernel<W, RP>, "adapter_shrink_kernel", dim3(c, s.tiles, n), THREADS, ShrinkMap<W, RP>::TOTAL, c, true, s.stream, a);
 }
 template <typename W, uint32_t RP>
 int expand(const Mat<W> &w, const __nv_bfloat16 *planes, const float *base, size_t base_pitch, float *y, size_t y_pitch, const Shape &s) {
     ExpandArgs<W> a = {w, planes, s.plane, s.lists, s.S, 1, base, base_pitch, y, y_pitch, s.status};
     const uint64_t blocks = (w.width + 127) / 128, tiles = (s.T + TM - 1) / TM;
-    a.blocks = (uint32_t)((blocks * tiles + 3 * SMS - 1) / (3 * SMS));
-    if (a.blocks > blocks) a.blocks = (uint32_t)blocks;
+    a.blocks = 1;
     return launch(adapter_expand_kernel<W, RP>, "adapter_expand_kernel", dim3((unsigned)((blocks + a.blocks - 1) / a.blocks), s.tiles), THREADS,
                   ExpandMap<W, RP>::TOTAL, 0, true, s.stream, a);
 }
@@ -1004,7 +1011,7 @@ int few(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, const uint32_t *
     constexpr int MOST = 16 / sizeof(W);
     auto runs_of = [&](uint32_t v) { return ad->k % v == 0 && ad->rank % v == 0 && (((uintptr_t)ad->a | (uintptr_t)ad->b) & (v * sizeof(W) - 1)) == 0; };
     const auto kernel = runs_of(MOST) ? adapter_few_kernel<W, MOST> : runs_of(4) ? adapter_few_kernel<W, 4> : adapter_few_kernel<W, 1>;
-    return launch(kernel, "adapter_few_kernel", dim3(FEW_CTAS, (unsigned)T), THREADS, 0, FEW_CTAS, false, stream, a);
+    return launch(kernel, "adapter_few_kernel", dim3(FEW_CTAS, (unsigned)T), THREADS, 0, FEW_CTAS, true, stream, a);
 }
 template <typename W, uint32_t RP>
 int forward(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, Rows base, float *y, size_t y_pitch, const Shape &s) {
@@ -1018,11 +1025,11 @@ int backward(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, Rows dy, Ro
                                   {mat_a<W>(ad), x.p, x.pitch, runs(x, s.T), (__nv_bfloat16 *)tune->h}};
     int rc;
     if ((rc = shrink<W, RP>(jobs, da ? 2 : 1, s))) return rc;
-    if (dx && (rc = expand<W, RP>(mat_a<W>(ad), jobs[0].planes, base.p, base.pitch, dx, dx_pitch, s))) return rc;
-    if (!da) return 0;
     const OuterJob outers[2] = {{x.p, x.pitch, (uint32_t)ad->k, jobs[1].x_fours, jobs[0].planes, da, (uint32_t)ad->k, 1, (uint32_t)((ad->k + 127) / 128)},
                                 {dy.p, dy.pitch, (uint32_t)ad->n, jobs[0].x_fours, jobs[1].planes, db, 1, ad->rank, (uint32_t)((ad->n + 127) / 128)}};
-    return outer<RP>(outers, s);
+    // dA and dB behind shrink, which has just read what they read
+    if (da && (rc = outer<RP>(outers, s))) return rc;
+    return dx ? expand<W, RP>(mat_a<W>(ad), jobs[0].planes, base.p, base.pitch, dx, dx_pitch, s) : 0;
 }
 
 #define BY_RANK(f, W, ...) (s.RP == 16 ? f<W, 16>(__VA_ARGS__) : s.RP == 32 ? f<W, 32>(__VA_ARGS__) : s.RP == 64 ? f<W, 64>(__VA_ARGS__) : f<W, 128>(__VA_ARGS__))
