@@ -30,7 +30,7 @@ extern "C" int qw4sh_allow_smem(const void *kernel, size_t smem);
 namespace {
 
 constexpr uint32_t THREADS = 256, TM = 128;                  // tokens per tile: tcgen05's M (shrink) or most N (expand)
-constexpr uint32_t KC = 64;                                  // shrink: columns per step
+constexpr uint32_t KC = 64, AHEAD = 1, OPS = 1;              // shrink: columns per step, steps that x is fetched ahead, stages of operands
 constexpr uint32_t TC = 64;                                  // outer: tokens per step
 
 // ---- PTX ------------------------------------------------------------------------------------------------------------------
@@ -157,10 +157,14 @@ template <> struct Four<float> {
         if (valid < 3) v.z = 0;
         if (valid < 4) v.w = 0;
     }
+    __device__ __forceinline__ void take(uint32_t addr) {
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    }
     __device__ __forceinline__ void put(uint32_t addr, uint32_t step) const { put_cut<3>(addr, step, v); }
 };
 template <typename H> struct Four16 {
     uint2 v;
+    __device__ __forceinline__ void take(uint32_t addr) { asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory"); }
     __device__ __forceinline__ void load4(const H *p) { v = *(const uint2 *)p; }
     __device__ __forceinline__ void load1(const H *q, uint32_t c, uint32_t last) {
         const uint16_t *row = (const uint16_t *)q;
@@ -182,6 +186,14 @@ template <> struct Four<__half> : Four16<__half> {
         put_cut<2>(addr, step, make_float4(a.x, a.y, b.x, b.y));
     }
 };
+// Copies to shared memory that the thread itself waits for: the first `there` of BYTES bytes, zeros behind them.
+template <uint32_t BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, uint32_t there) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(there), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
 // How many of four places from c on lie before `end`.
 __device__ __forceinline__ int places(uint32_t c, uint32_t end) { return c < end ? (int)min(4u, end - c) : 0; }
 
@@ -192,12 +204,13 @@ template <typename W> struct Mat { const W *p; uint64_t slot; uint32_t rank, wid
 // A run of LEN columns of a slot's matrix (rank padded to RP) on its way into the operand tiles Wide (RP x LEN) or Tall (LEN x RP).
 // Where runs of four lie on their boundaries a thread keeps the places it reads in such runs and moves them on from run to run.
 template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
-    static constexpr uint32_t UNITS = RP * LEN / 4 / THREADS, PLANES = Four<W>::PLANES;
+    static constexpr uint32_t ALL = RP * LEN / 4, UNITS = (ALL + THREADS - 1) / THREADS, PLANES = Four<W>::PLANES;
     using Wide = Tile<RP, LEN, PLANES>;
     using Tall = Tile<LEN, RP, PLANES>;
     static constexpr uint32_t BYTES = Wide::BYTES > Tall::BYTES ? Wide::BYTES : Tall::BYTES;
     Four<W> v[UNITS];
     uint32_t at[UNITS];
+    static __device__ __forceinline__ bool idle() { return ALL < THREADS && threadIdx.x >= ALL; }           // fewer runs of four than threads
     static __device__ __forceinline__ uint32_t wide_r(uint32_t i) { return (threadIdx.x + i * THREADS) / (LEN / 4); }
     static __device__ __forceinline__ uint32_t wide_c(uint32_t i) { return (threadIdx.x + i * THREADS) % (LEN / 4) * 4; }
     static __device__ __forceinline__ uint32_t tall_c(uint32_t i) { return (threadIdx.x + i * THREADS) / (RP / 4); }
@@ -209,6 +222,7 @@ template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
     }
     // columns c0 .. c0 + LEN of w, which end at `end`
     __device__ __forceinline__ void load(const Mat<W> &m, const W *w, uint32_t c0, uint32_t end) {
+        if (idle()) return;
         if (m.fours && c0 + LEN <= end) {
             const uint32_t step = m.wide ? LEN / 4 : LEN / 4 * m.rank;
 #pragma unroll
@@ -229,11 +243,27 @@ template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
             }
         }
     }
+    // the same by way of the thread's own places in shared memory, UNITS of them `stride` bytes apart; only where m.fours
+    __device__ __forceinline__ void copy(const Mat<W> &m, const W *w, uint32_t c0, uint32_t end, uint32_t to, uint32_t stride) {
+        if (idle()) return;
+        const uint32_t step = m.wide ? LEN / 4 : LEN / 4 * m.rank;
+#pragma unroll
+        for (uint32_t i = 0; i < UNITS; i++) {
+            const bool there = m.wide ? c0 + wide_c(i) < end : c0 + tall_c(i) < end;
+            copy_async<4 * sizeof(W)>(to + i * stride, there ? w + (uint64_t)at[i] * 4 : w, there ? 4 * sizeof(W) : 0);
+            at[i] += step;
+        }
+    }
+    __device__ __forceinline__ void take(uint32_t from, uint32_t stride) {
+#pragma unroll
+        for (uint32_t i = 0; i < UNITS; i++) v[i].take(from + i * stride);
+    }
     __device__ __forceinline__ void set(uint32_t i, const Four<W> &f) {
 #pragma unroll
         for (uint32_t j = 0; j < UNITS; j++) if (i == j) v[j] = f;
     }
     __device__ __forceinline__ void put(const Mat<W> &m, uint32_t c0, uint32_t end, uint32_t addr) {
+        if (idle()) return;
         if (m.rank != RP || c0 + LEN > end)
 #pragma unroll
             for (uint32_t i = 0; i < UNITS; i++) {
@@ -264,15 +294,15 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
     uint32_t *mine = counts + warp * G, *starts = counts + 32 * G;
     grid_go();                                               // the tiles' CTAs may take their places
     grid_wait();
-    constexpr uint32_t AHEAD = 8;                            // loads in flight
-    uint32_t s[AHEAD], same[AHEAD];
+    constexpr uint32_t LOADS = 8;                            // in flight
+    uint32_t s[LOADS], same[LOADS];
     auto fetch = [&](uint32_t t0) {
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; i++) s[i] = t0 + 32 * i + lane < end ? ids[t0 + 32 * i + lane] : 0;
+        for (uint32_t i = 0; i < LOADS; i++) s[i] = t0 + 32 * i + lane < end ? ids[t0 + 32 * i + lane] : 0;
     };
     auto match = [&](uint32_t t0) {
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; i++) {
+        for (uint32_t i = 0; i < LOADS; i++) {
             const bool there = t0 + 32 * i + lane < end;
             if (there && s[i] >= S && s[i] != QW4CU_NO_ADAPTER) atomicOr(status, QW4SH_ERR_BOUNDS);
             s[i] = there ? min(s[i], S) : 0xffffffffu;
@@ -283,10 +313,10 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
     for (uint32_t i = threadIdx.x; i < 32 * G; i += 1024) counts[i] = 0;
     match(first);
     __syncthreads();
-    for (uint32_t t0 = first; t0 < end; t0 += 32 * AHEAD) {
+    for (uint32_t t0 = first; t0 < end; t0 += 32 * LOADS) {
         if (t0 != first) { fetch(t0); match(t0); }
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; i++) {
+        for (uint32_t i = 0; i < LOADS; i++) {
             if (s[i] <= S && __ffs(same[i]) - 1 == (int)lane) mine[s[i]] += __popc(same[i]);
             __syncwarp();
         }
@@ -331,11 +361,11 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
         if (g == S) *n_tiles = tile;
     }
     __syncthreads();
-    if (per > 32 * AHEAD) { fetch(first); match(first); }    // else they are still there
-    for (uint32_t t0 = first; t0 < end; t0 += 32 * AHEAD) {
+    if (per > 32 * LOADS) { fetch(first); match(first); }    // else they are still there
+    for (uint32_t t0 = first; t0 < end; t0 += 32 * LOADS) {
         if (t0 != first) { fetch(t0); match(t0); }
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; i++) {
+        for (uint32_t i = 0; i < LOADS; i++) {
             const bool there = s[i] <= S;
             const uint32_t before = there ? mine[s[i]] : 0;
             __syncwarp();
@@ -421,12 +451,16 @@ template <typename W> struct ShrinkArgs {
 template <typename W, uint32_t RP> struct ShrinkMap {
     using X = Tile<TM, KC, 3>;                               // rows tokens: K-major
     using Run = MatRun<W, RP, KC>;                           // Wide: K-major, Tall: MN-major
-    static constexpr uint32_t ORDER = 64, STAGE = ORDER + TM * 4, W_AT = STAGE + X::BYTES;
+    static constexpr uint32_t XU = TM * KC / 4 / THREADS;    // runs of four values of x per thread and step
+    static constexpr uint32_t W_UNIT = THREADS * 4 * sizeof(W), SLOT = XU * THREADS * 16 + Run::UNITS * W_UNIT;
+    static constexpr uint32_t OPERANDS = X::BYTES + Run::BYTES;
+    static constexpr uint32_t ORDER = 64, STAGE = ORDER + TM * 4, RING = STAGE + OPS * OPERANDS, END = RING + AHEAD * SLOT;
     static constexpr uint32_t PITCH = RP + 4;                // floats per row of the exchanged accumulators
-    static constexpr uint32_t END = W_AT + Run::BYTES, ACC_END = STAGE + TM * PITCH * 4, TOTAL = END > ACC_END ? END : ACC_END;
+    static constexpr uint32_t ACC_END = STAGE + TM * PITCH * 4, TOTAL = END > ACC_END ? END : ACC_END;
 };
 
-// One operand stage and no second one: three CTAs to an SM cover each other's waits, and two stages would leave room for one or two.
+// Values come in by asynchronous copies, AHEAD steps before they are cut, each thread's own into places of its own: no barrier, no register and no line
+// of L1 holds them meanwhile (through registers an SM had half as many bytes under way).
 template <typename W, uint32_t RP>
 __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel(const __grid_constant__ ShrinkArgs<W> a) {
     namespace cg = cooperative_groups;
@@ -441,9 +475,9 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
     if (blockIdx.y >= *a.lists.n_tiles) return;              // the same for all CTAs of a cluster
     const ATile t = a.lists.tiles[blockIdx.y];
     if (t.slot >= a.slots) return;
-    if (tid == 0) bar_init(base);
+    if (tid < 2) bar_init(base + 8 * tid);
     if (warp == 0) tc_alloc(base + 32, Sums<RP>::COLS);
-    if (tid < TM) order[tid] = a.lists.order[t.first + min(tid, t.rows - 1)];      // rows that are not there: the last one again, unused
+    if (tid < TM) order[tid] = a.lists.order[t.first + min(tid, t.rows - 1)];
     tc_before();
     __syncthreads();
     tc_after();
@@ -453,49 +487,69 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
     const uint32_t steps = uniform((c_end - c_first + KC - 1) / KC);
     const W *w = m.p + t.slot * m.slot;
 
-    constexpr uint32_t XU = TM * KC / 4 / THREADS, ROWS = THREADS / (KC / 4);        // runs of four values per thread, rows from one to the next
-    const uint32_t x_row = tid / (KC / 4), x_col = tid % (KC / 4) * 4;
-    Four<float> xv[XU];
+    constexpr uint32_t XU = M::XU, ROWS = THREADS / (KC / 4);                        // rows from one run of four to the thread's next
+    const uint32_t x_row = tid / (KC / 4), x_col = tid % (KC / 4) * 4, mine = base + M::RING + tid * 16, mine_w = base + M::RING + XU * THREADS * 16 + tid * 4 * sizeof(W);
     uint32_t x_at[XU];                                       // places in runs of four
     typename M::Run wv;
 #pragma unroll
     for (uint32_t i = 0; i < XU; i++) x_at[i] = (uint32_t)((order[x_row + i * ROWS] * job.pitch + c_first + x_col) / 4);
     wv.begin(m, c_first);
     const float *x = job.x;
-    auto fetch = [&](uint32_t c0) {
-        if (job.x_fours && c0 + KC <= c_end) {
+    auto copy = [&](uint32_t s) {
+        if (s < steps) {
+            const uint32_t c = c_first + s * KC + x_col, slot = s % AHEAD * M::SLOT;
+            const uint32_t valid = places(c, c_end);
+            if (job.x_fours) {
 #pragma unroll
-            for (uint32_t i = 0; i < XU; i++) { xv[i].load4(x + (uint64_t)x_at[i] * 4); x_at[i] += KC / 4; }
-        } else {
+                for (uint32_t i = 0; i < XU; i++) {
+                    const bool there = x_row + i * ROWS < t.rows && valid;
+                    copy_async<16>(mine + slot + i * THREADS * 16, there ? x + (uint64_t)x_at[i] * 4 : x, there ? 4 * valid : 0);
+                    x_at[i] += KC / 4;
+                }
+            } else {
+#pragma unroll 1
+                for (uint32_t i = 0; i < XU; i++) {
+                    const float *row = x + order[x_row + i * ROWS] * job.pitch;
 #pragma unroll
-            for (uint32_t i = 0; i < XU; i++) xv[i].load1(x + order[x_row + i * ROWS] * job.pitch, c0 + x_col, c_end - 1);
+                    for (uint32_t j = 0; j < 4; j++) {
+                        const bool there = x_row + i * ROWS < t.rows && j < valid;
+                        copy_async<4>(mine + slot + i * THREADS * 16 + 4 * j, there ? row + c + j : x, there ? 4 : 0);
+                    }
+                }
+            }
+            if (m.fours) wv.copy(m, w, c_first + s * KC, c_end, mine_w + slot, M::W_UNIT);
         }
-        wv.load(m, w, c0, c_end);
+        copies_commit();
     };
-    if (steps) fetch(c_first);
+#pragma unroll
+    for (uint32_t s = 0; s < AHEAD; s++) copy(s);
     const uint32_t idesc = idesc_of(TM, RP, false, !m.wide);
     for (uint32_t s = 0; s < steps; s++) {
-        const uint32_t c0 = c_first + s * KC;
-        if (s) bar_wait(base, (s - 1) & 1, a.status);
-        if (c0 + KC > c_end)
+        const uint32_t c0 = c_first + s * KC, slot = s % AHEAD * M::SLOT, at = base + M::STAGE + s % OPS * M::OPERANDS, wat = at + M::X::BYTES, bar = base + 8 * (s % OPS);
+        copies_wait<AHEAD - 1>();
+        if (s >= OPS) bar_wait(bar, (s / OPS - 1) & 1, a.status);
 #pragma unroll
-            for (uint32_t i = 0; i < XU; i++) xv[i].keep(places(c0 + x_col, c_end));
-#pragma unroll
-        for (uint32_t i = 0; i < XU; i++) xv[i].put(base + M::STAGE + M::X::at(x_row + i * ROWS, x_col), M::X::PLANE);
-        wv.put(m, c0, c_end, base + M::W_AT);
+        for (uint32_t i = 0; i < XU; i++) {
+            Four<float> xv;
+            xv.take(mine + slot + i * THREADS * 16);
+            xv.put(at + M::X::at(x_row + i * ROWS, x_col), M::X::PLANE);
+        }
+        if (m.fours) wv.take(mine_w + slot, M::W_UNIT); else wv.load(m, w, c0, c_end);
+        wv.put(m, c0, c_end, wat);
+        copy(s + AHEAD);
         fence_async();
         __syncthreads();
         if (warp == 0) {
             tc_after();
             const uint32_t leader = elect();                 // the thread whose products the commit answers for
-            if (m.wide) step_mma<typename M::X, typename M::Run::Wide, 3, M::Run::PLANES, false, false, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::W_AT, idesc, s == 0, leader);
-            else step_mma<typename M::X, typename M::Run::Tall, 3, M::Run::PLANES, false, true, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::W_AT, idesc, s == 0, leader);
-            if (leader) tc_commit(base);
+            if (m.wide) step_mma<typename M::X, typename M::Run::Wide, 3, M::Run::PLANES, false, false, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, at, wat, idesc, s == 0, leader);
+            else step_mma<typename M::X, typename M::Run::Tall, 3, M::Run::PLANES, false, true, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, at, wat, idesc, s == 0, leader);
+            if (leader) tc_commit(bar);
             __syncwarp();
         }
-        if (s + 1 < steps) fetch(c0 + KC);                   // behind the products: the SM takes no more loads than it has lines for, and makes them wait
     }
-    if (steps) bar_wait(base, (steps - 1) & 1, a.status);
+    copies_wait<0>();
+    if (steps) bar_wait(base + 8 * ((steps - 1) % OPS), ((steps - 1) / OPS) & 1, a.status);
     tc_after();
     grid_go();                                               // not before: CTAs of the next launch would crowd onto the SMs that are done first
     // accumulators to shared memory, summed over the cluster's CTAs in their order, scaled, cut and stored
@@ -967,9 +1021,9 @@ int make_lists(const QW4ShTune *tune, const QW4CuAdapters *ad, const uint32_t *s
 }
 
 // As many CTAs to a tile as give every SM two, a run of 128 columns each at least.
-uint32_t cluster_of(uint64_t items, uint64_t length, uint32_t least, uint32_t most = 8) {
+uint32_t cluster_of(uint64_t items, uint64_t length, uint32_t least, uint32_t ctas) {
     uint32_t c = 1;
-    while (c < most && items * c < 2 * SMS && length / (2 * c) >= least) c *= 2;
+    while (c < 8 && items * 2 * c <= ctas && length / (2 * c) >= least) c *= 2;
     return c;
 }
 
@@ -979,13 +1033,13 @@ int shrink(const ShrinkJob<W> *jobs, uint32_t n, const Shape &s) {
     uint64_t width = 0;
     for (uint32_t i = 0; i < n; i++) { a.job[i] = jobs[i]; if (jobs[i].w.width > width) width = jobs[i].w.width; }
     a.lists = s.lists; a.scale = s.scale; a.plane = s.plane; a.slots = s.S; a.status = s.status;
-    const uint32_t c = cluster_of((uint64_t)(s.T + TM - 1) / TM * n, width, 128, s.T > 4096 ? 4 : 8);
+    const uint32_t c = cluster_of((uint64_t)(s.T + TM - 1) / TM * n, width, 128, 2 * SMS);
     return launch(adapter_shrink_kernel<W, RP>, "adapter_shrink_kernel", dim3(c, s.tiles, n), THREADS, ShrinkMap<W, RP>::TOTAL, c, true, s.stream, a);
 }
 template <typename W, uint32_t RP>
 int expand(const Mat<W> &w, const __nv_bfloat16 *planes, const float *base, size_t base_pitch, float *y, size_t y_pitch, const Shape &s) {
     ExpandArgs<W> a = {w, planes, s.plane, s.lists, s.S, 1, base, base_pitch, y, y_pitch, s.status};
-    const uint64_t blocks = (w.width + 127) / 128, tiles = (s.T + TM - 1) / TM;
+    const uint64_t blocks = (w.width + 127) / 128;
     a.blocks = 1;
     return launch(adapter_expand_kernel<W, RP>, "adapter_expand_kernel", dim3((unsigned)((blocks + a.blocks - 1) / a.blocks), s.tiles), THREADS,
                   ExpandMap<W, RP>::TOTAL, 0, true, s.stream, a);
@@ -994,7 +1048,7 @@ template <uint32_t RP>
 int outer(const OuterJob *jobs, const Shape &s) {
     OuterArgs a = {{jobs[0], jobs[1]}, s.lists, s.plane, s.R, s.status};
     const uint32_t blocks = jobs[0].blocks + jobs[1].blocks;
-    const uint32_t c = cluster_of((uint64_t)blocks * ((s.T + 1023) / 1024 < s.S ? (s.T + 1023) / 1024 : s.S), s.T, TC);
+    const uint32_t c = cluster_of((uint64_t)blocks * ((s.T + 1023) / 1024 < s.S ? (s.T + 1023) / 1024 : s.S), s.T, TC, 4 * SMS);
     return launch(adapter_outer_kernel<RP>, "adapter_outer_kernel", dim3(c, blocks, s.S), THREADS, OuterMap<RP>::TOTAL, c, true, s.stream, a);
 }
 
