@@ -280,6 +280,8 @@ class MoeApi:
             "qw4cu_tune_work_reset": ([P, E], C.c_int),
             "qw4cu_adapter_forward_device": ([P, P, C.c_size_t, P, P, C.c_size_t, P, C.c_size_t, C.c_size_t, P, P], C.c_int),
             "qw4cu_adapter_backward_device": ([P, P, C.c_size_t, P, P, C.c_size_t, P, C.c_size_t, P, C.c_size_t, P, P, C.c_size_t, P, P], C.c_int),
+            "qw4cu_moe_route_adapted_device": ([P, P, C.c_size_t, P, P, P, P, P, P, P, P], C.c_int),
+            "qw4cu_moe_forward_adapted_device": ([P, P, P, C.c_size_t, P, P, P, P, P, P, P, P], C.c_int),
             "qw4cu_balance_forward_device": ([P, P, C.c_size_t, P, P, C.c_size_t, P, P, P, P, P], C.c_int),
             "qw4cu_balance_backward_device": ([P, P, C.c_size_t, P, P, C.c_size_t, P, C.c_float, P, P, C.c_size_t, P, P], C.c_int),
         }

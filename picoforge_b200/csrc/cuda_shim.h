@@ -46,6 +46,8 @@ typedef struct {
  * the minima, and what undoes the scale (one float per row, or per 128 columns of an activation). */
 typedef struct { void *hi, *lo, *sum_hi, *sum_lo; float *scale; } QW4ShSplit;
 
+typedef struct QW4ShTune QW4ShTune;
+
 /* Device scratch of one workspace, sized for `cap` tokens. */
 typedef struct {
     size_t cap;
@@ -89,6 +91,12 @@ typedef struct {
     /* set per call, NULL otherwise: pinned host words [4] into which the one-kernel decode path copies the status
      * words when its last CTA leaves (the host forward then needs no copy of them) */
     uint32_t *status_mirror;
+    /* set per call, NULL otherwise: adapters that are added to the router's logits before they are routed (with the slots of
+     * the tokens and the scratch that they need), and where the logits that were routed are copied to, [tokens, experts] */
+    const QW4CuAdapters *router_adapters;
+    const uint32_t *router_slots;
+    const QW4ShTune *router_tune;
+    float *logits_out;
 } QW4ShWork;
 
 enum { QW4SH_ERR_NONFINITE = 1u, QW4SH_ERR_BOUNDS = 2u, QW4SH_ERR_STATE = 4u };
@@ -240,8 +248,8 @@ int qw4sh_observed_forward(const QW4ShLayer *layer, const QW4ShWork *work, const
                            size_t x_host_pitch, size_t token0, QW4MoeObserver observer, void *ctx);
 int qw4sh_route_forward(const QW4ShLayer *layer, const QW4ShWork *work, const float *x, size_t tokens, int router_mode);
 /* Adapters and balance loss (adapters.cu, balance.cu): device scratch of one QW4CuTuneWork. */
-typedef struct {
-    uint32_t *status;             /* [4]: error bits, lowest bad row */
+struct QW4ShTune {
+    uint32_t *status;             /* [4]: error bits, lowest bad row, whether this forward pass of the loss met one */
     /* balance loss: sums over the CTAs of a launch, zero between launches */
     unsigned long long *prob_sums;    /* [experts] units of 2^-40 */
     uint32_t *counts;             /* [experts + 1], and one ticket behind them */
@@ -251,8 +259,12 @@ typedef struct {
     uint32_t *n_tiles;
     /* A x and B^T dy of every token, in that order, cut in three bf16 values */
     void *h, *g;                  /* [3][qw4sh_adapter_rows(tokens, slots) x qw4sh_adapter_rank(rank)] */
-} QW4ShTune;
+};
 size_t qw4sh_adapter_rows(size_t tokens, uint32_t slots);
+/* tune_host.c: the scratch of a workspace for adapters beside a projection of k inputs and n outputs, after the checks of
+ * qw4cu_adapter_forward_device on what is given here. */
+Qwen4Status qw4tune_beside(const QW4CuAdapters *adapters, size_t k, size_t n, const uint32_t *slots, size_t tokens, QW4CuTuneWork *work,
+                           const QW4ShTune **tune, Qwen4Error *err);
 size_t qw4sh_adapter_tiles(size_t tokens, uint32_t slots);
 uint32_t qw4sh_adapter_rank(uint32_t rank);
 int qw4sh_balance_forward(const QW4ShTune *tune, uint32_t experts, uint32_t k, const float *logits, size_t pitch, const uint32_t *ids,

@@ -1648,7 +1648,7 @@ static int aux_stream(cudaStream_t *stream, cudaEvent_t **events) {
 }
 
 static bool takes_fused(const QW4ShLayer *layer, const QW4ShWork *work, const float *x, const float *y, size_t tokens) {
-    return g_only_step < 0 && g_expert_path != 0 && !work->routed && qw4sh_fused_supported(layer, tokens, x, y, sm_count());
+    return g_only_step < 0 && g_expert_path != 0 && !work->routed && !work->router_adapters && !work->logits_out && qw4sh_fused_supported(layer, tokens, x, y, sm_count());
 }
 
 // Whether a forward of this batch would run as the one-kernel decode path (which writes every y element exactly once
@@ -1660,6 +1660,17 @@ extern "C" int qw4sh_takes_fused(const QW4ShLayer *layer, const QW4ShWork *work,
 __global__ void __launch_bounds__(256) hc_add_kernel(const float *__restrict__ y, uint32_t hidden, HcAdd hc, uint32_t *status) {
     const uint32_t t = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
     if (c < hidden && !hc_add(hc, t, c, hidden, y[(uint64_t)t * hidden + c])) atomicOr(status, QW4SH_ERR_NONFINITE);
+}
+
+// The router's logits are there: the requests' adapters on top of them, and a copy for who asked for one.
+static int adapt_logits(const QW4ShLayer *layer, const QW4ShWork *work, const float *x, size_t tokens, cudaStream_t stream) {
+    const size_t E = layer->experts;
+    if (work->router_adapters) {
+        const int rc = qw4sh_adapter_forward(work->router_tune, work->router_adapters, x, layer->hidden, work->router_slots, work->logits, E, work->logits, E, tokens, stream);
+        if (rc) return rc;
+    }
+    if (work->logits_out) CU(cudaMemcpyAsync(work->logits_out, work->logits, tokens * E * 4, cudaMemcpyDeviceToDevice, stream));
+    return 0;
 }
 
 static int layer_launches(const QW4ShLayer *layer, const QW4ShWork *work, const float *x, float *y, size_t tokens,
@@ -1726,6 +1737,7 @@ static int layer_launches(const QW4ShLayer *layer, const QW4ShWork *work, const 
         return STEP(8) ? products(1, true, side) : 0;
     };
     if (STEP(0) && (rc = launch_router(layer, x, tokens, work->logits, work->shared_logit, work->status, router_mode, stream))) return rc;
+    if ((rc = adapt_logits(layer, work, x, tokens, stream))) return rc;
     STAGE_MARK();
     if (listed) {
         RouteArgs a = {};
@@ -1814,6 +1826,7 @@ extern "C" int qw4sh_route_forward(const QW4ShLayer *layer, const QW4ShWork *wor
     cudaStream_t stream = (cudaStream_t)work->stream;
     int rc;
     if ((rc = launch_router(layer, x, tokens, work->logits, work->shared_logit, work->status, router_mode, stream))) return rc;
+    if ((rc = adapt_logits(layer, work, x, tokens, stream))) return rc;
     return qw4sh_route(layer->experts, layer->top_k, layer->norm, work->logits, layer->experts, tokens, work->probs, work->ids,
                        work->weights, work->status, stream);
 }
@@ -2076,7 +2089,8 @@ extern "C" int qw4sh_layer_forward(const QW4ShLayer *layer, const QW4ShWork *wor
     // the one-kernel decode path is one launch already, chained to its neighbours by programmatic stream serialisation
     if (takes_fused(layer, work, x, y, tokens)) return layer_launches(layer, work, x, y, tokens, ids_out, weights_out, router_mode, false);
     if (!g_graph_mode || !cache) return layer_launches(layer, work, x, y, tokens, ids_out, weights_out, router_mode, false);
-    if (work->hc_residual) return layer_launches(layer, work, x, y, tokens, ids_out, weights_out, router_mode, false);   // not replayed
+    if (work->hc_residual || work->router_adapters || work->logits_out)
+        return layer_launches(layer, work, x, y, tokens, ids_out, weights_out, router_mode, false);   // not replayed
     const bool same = cache->layer == layer && cache->x == x && cache->y == y && cache->ids == ids_out &&
                       cache->weights == weights_out && cache->tokens == tokens && cache->mode == router_mode;
     if (same && cache->exec) {

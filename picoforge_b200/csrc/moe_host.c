@@ -518,6 +518,30 @@ Qwen4Status qw4cu_moe_route_device(const Qwen4Moe *m, const float *x_dev, size_t
     if (tokens && weights_dev && qw4sh_memcpy2d_async(weights_dev, bytes, w->d.weights, bytes, bytes, 1, 2, w->d.stream)) return cuda_failure(err, "weights copy");
     return report(err, QW4_OK, "");
 }
+/* ---- adapters beside the router ------------------------------------------------------------ */
+/* One of the two device calls with the requests' adapters on the router's logits and a copy of the logits that were routed. */
+static Qwen4Status adapted(const Qwen4Moe *m, const float *x_dev, float *y_dev, bool route_only, size_t tokens, const QW4CuAdapters *adapters,
+                           const uint32_t *slots_dev, QW4CuTuneWork *tune, float *logits_dev, uint32_t *ids_dev, float *weights_dev,
+                           Qwen4MoeWork *w, Qwen4Error *err) {
+    TRY(piece_checks(m, w, tokens, err));
+    const QW4ShTune *scratch = NULL;
+    if (adapters) TRY(qw4tune_beside(adapters, m->c.hidden_size, m->c.experts, slots_dev, tokens, tune, &scratch, err));
+    w->d.router_adapters = tokens ? adapters : NULL; w->d.router_slots = slots_dev; w->d.router_tune = scratch; w->d.logits_out = tokens ? logits_dev : NULL;
+    const Qwen4Status st = route_only ? qw4cu_moe_route_device(m, x_dev, tokens, ids_dev, weights_dev, w, err)
+                                      : qw4cu_moe_forward_device(m, x_dev, y_dev, tokens, ids_dev, weights_dev, w, err);
+    w->d.router_adapters = NULL; w->d.router_slots = NULL; w->d.router_tune = NULL; w->d.logits_out = NULL;
+    return st;
+}
+Qwen4Status qw4cu_moe_route_adapted_device(const Qwen4Moe *m, const float *x_dev, size_t tokens, const QW4CuAdapters *adapters, const uint32_t *slots_dev,
+                                           QW4CuTuneWork *tune, float *logits_dev, uint32_t *ids_dev, float *weights_dev, Qwen4MoeWork *w, Qwen4Error *err) {
+    return adapted(m, x_dev, NULL, true, tokens, adapters, slots_dev, tune, logits_dev, ids_dev, weights_dev, w, err);
+}
+Qwen4Status qw4cu_moe_forward_adapted_device(const Qwen4Moe *m, const float *x_dev, float *y_dev, size_t tokens, const QW4CuAdapters *adapters,
+                                             const uint32_t *slots_dev, QW4CuTuneWork *tune, float *logits_dev, uint32_t *ids_dev, float *weights_dev,
+                                             Qwen4MoeWork *w, Qwen4Error *err) {
+    return adapted(m, x_dev, y_dev, false, tokens, adapters, slots_dev, tune, logits_dev, ids_dev, weights_dev, w, err);
+}
+
 /* ---- expert parallelism ------------------------------------------------------------------ */
 struct QW4CuEp { QW4ShEp *shim; };
 

@@ -186,6 +186,18 @@ static Qwen4Status check_adapters(const QW4CuAdapters *ad, const QW4CuTuneWork *
     return QW4_OK;
 }
 
+Qwen4Status qw4tune_beside(const QW4CuAdapters *ad, size_t k, size_t n, const uint32_t *slots, size_t tokens, QW4CuTuneWork *w,
+                           const QW4ShTune **tune, Qwen4Error *err) {
+    void *stream;
+    Bytes at;
+    TRY(usable(w, tokens, &stream, err));
+    TRY(check_adapters(ad, w, &at, &at, &at, err));
+    if (ad->k != k || ad->n != n) return answer(err, QW4_SHAPE, "adapters of another projection");
+    if (tokens) VIEW(slots, 1, tokens * 4, tokens * 4, 4, &at);
+    *tune = &w->d;
+    return QW4_OK;
+}
+
 Qwen4Status qw4cu_adapter_forward_device(const QW4CuAdapters *ad, const float *x, size_t x_pitch, const uint32_t *slots, const float *base,
                                          size_t base_pitch, float *y, size_t y_pitch, size_t tokens, QW4CuTuneWork *w, Qwen4Error *err) {
     void *stream;

@@ -49,6 +49,16 @@ class TuneWork:
             C.byref(adapters), x, x_pitch or k4, slots, dy, dy_pitch or n4, base, base_pitch or k4, dx, dx_pitch or k4, da, db, tokens,
             self.handle, self._err))
 
+    def route(self, layer, adapters, x, slots, tokens, logits=None, ids=None, weights=None):
+        """Routes of a `MoeLayer` with adapters (or None) beside its router; logits [tokens, experts]: what was routed."""
+        self._check(self.api.lib.qw4cu_moe_route_adapted_device(
+            layer.moe, x, tokens, C.byref(adapters) if adapters else None, slots, self.handle, logits, ids, weights, layer.work, self._err))
+
+    def layer_forward(self, layer, adapters, x, slots, y, tokens, logits=None, ids=None, weights=None):
+        """The whole layer on those routes."""
+        self._check(self.api.lib.qw4cu_moe_forward_adapted_device(
+            layer.moe, x, y, tokens, C.byref(adapters) if adapters else None, slots, self.handle, logits, ids, weights, layer.work, self._err))
+
     def balance_forward(self, config, logits, ids, mask, tokens, counts, prob_sums, loss, logits_pitch=0):
         self._check(self.api.lib.qw4cu_balance_forward_device(
             C.byref(config), logits, logits_pitch or config.experts * 4, ids, mask, tokens, counts, prob_sums, loss, self.handle, self._err))
