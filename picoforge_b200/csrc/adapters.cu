@@ -19,6 +19,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <pthread.h>
 #include <stdint.h>
 
 #include "cuda_shim.h"
@@ -572,10 +573,12 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
         const uint32_t row = part * rows + u / (2 * RP) * 8 + (u >> 1 & 7), c = (u >> 4) % (RP / 8) * 8 + (u & 1) * 4;
         if (row >= rows16) break;
         float4 v[8], sum = make_float4(0, 0, 0, 0);
+        for (uint32_t q = 0; q < parts; q += 8) {
 #pragma unroll
-        for (uint32_t p = 0; p < 8; p++) if (p < parts) v[p] = *(const float4 *)(cluster.map_shared_rank(acc, p) + row * M::PITCH + c);
+            for (uint32_t p = 0; p < 8; p++) if (q + p < parts) v[p] = *(const float4 *)(cluster.map_shared_rank(acc, q + p) + row * M::PITCH + c);
 #pragma unroll
-        for (uint32_t p = 0; p < 8; p++) if (p < parts) { sum.x += v[p].x; sum.y += v[p].y; sum.z += v[p].z; sum.w += v[p].w; }
+            for (uint32_t p = 0; p < 8; p++) if (q + p < parts) { sum.x += v[p].x; sum.y += v[p].y; sum.z += v[p].z; sum.w += v[p].w; }
+        }
         const bool there = row < t.rows;
         sum = make_float4(there ? sum.x * scale : 0, there ? sum.y * scale : 0, there ? sum.z * scale : 0, there ? sum.w * scale : 0);
         __nv_bfloat16 *to = job.planes + (uint64_t)((t.first + row) >> 3) * (8 * RP) + (c >> 3) * 64 + (row & 7) * 8 + (c & 7);
@@ -838,7 +841,7 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
 // One cluster of eight CTAs to a token, whatever its slot: A x with a run of columns of x to each CTA, the eight partial sums of every r
 // to all of them (distributed shared memory), B h with a run of y's columns to each.  Everything is read once and one launch is all
 // there is.  What bounds it is latency: the id, then A, the exchange, then the sum; B and base are on their way meanwhile.
-constexpr uint32_t FEW_CTAS = 8, FEW_TOKENS = 128;
+constexpr uint32_t FEW_CTAS = 8;
 
 template <typename W> struct FewArgs {
     const W *a, *b;
@@ -1002,6 +1005,33 @@ int launch(void (*kernel)(A...), const char *name, dim3 grid, uint32_t threads, 
 bool fours(const void *p, size_t step, size_t element) { return (uintptr_t)p % (4 * element) == 0 && step % 4 == 0; }
 
 constexpr uint32_t SMS = 148;
+
+// Most CTAs to a cluster of this kernel: sixteen where the device has room for one (eight is what every device promises).
+uint32_t most_ctas(const void *kernel, size_t smem) {
+    static struct { const void *kernel; int device; uint32_t most; } have[64];
+    static uint32_t n = 0;
+    static pthread_mutex_t lock = PTHREAD_MUTEX_INITIALIZER;
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 8;
+    pthread_mutex_lock(&lock);
+    uint32_t i = 0, most = 8;
+    while (i < n && (have[i].kernel != kernel || have[i].device != device)) i++;
+    if (i < n) most = have[i].most;
+    else {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(16); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension; attr.val.clusterDim.x = 16; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr; cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess && !qw4sh_allow_smem(kernel, smem) &&
+            cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters >= 4) most = 16;
+        (void)cudaGetLastError();
+        if (n < 64) { have[n].kernel = kernel; have[n].device = device; have[n++].most = most; }
+    }
+    pthread_mutex_unlock(&lock);
+    return most;
+}
 struct Shape {
     uint32_t T, S, R, RP, tiles;                             // tiles: most that there can be
     Lists lists;
@@ -1020,10 +1050,10 @@ int make_lists(const QW4ShTune *tune, const QW4CuAdapters *ad, const uint32_t *s
                   tune->offsets, (ATile *)tune->tiles, tune->n_tiles, tune->status);
 }
 
-// As many CTAs to a tile as give every SM two, a run of 128 columns each at least.
-uint32_t cluster_of(uint64_t items, uint64_t length, uint32_t least, uint32_t ctas) {
+// CTAs to a cluster: as many as `ctas` has room for, with a run of `least` each at least.
+uint32_t cluster_of(uint64_t items, uint64_t length, uint32_t least, uint32_t ctas, uint32_t most = 8) {
     uint32_t c = 1;
-    while (c < 8 && items * 2 * c <= ctas && length / (2 * c) >= least) c *= 2;
+    while (c < most && items * 2 * c <= ctas && length / (2 * c) >= least) c *= 2;
     return c;
 }
 
@@ -1033,7 +1063,7 @@ int shrink(const ShrinkJob<W> *jobs, uint32_t n, const Shape &s) {
     uint64_t width = 0;
     for (uint32_t i = 0; i < n; i++) { a.job[i] = jobs[i]; if (jobs[i].w.width > width) width = jobs[i].w.width; }
     a.lists = s.lists; a.scale = s.scale; a.plane = s.plane; a.slots = s.S; a.status = s.status;
-    const uint32_t c = cluster_of((uint64_t)(s.T + TM - 1) / TM * n, width, 128, 2 * SMS);
+    const uint32_t c = cluster_of((uint64_t)(s.T + TM - 1) / TM * n, width, 128, 2 * SMS, most_ctas((const void *)adapter_shrink_kernel<W, RP>, ShrinkMap<W, RP>::TOTAL));
     return launch(adapter_shrink_kernel<W, RP>, "adapter_shrink_kernel", dim3(c, s.tiles, n), THREADS, ShrinkMap<W, RP>::TOTAL, c, true, s.stream, a);
 }
 template <typename W, uint32_t RP>
@@ -1106,7 +1136,10 @@ extern "C" size_t qw4sh_adapter_tiles(size_t tokens, uint32_t slots) {
 extern "C" int qw4sh_adapter_forward(const QW4ShTune *tune, const QW4CuAdapters *ad, const float *x, size_t x_pitch, const uint32_t *slots,
                                      const float *base, size_t base_pitch, float *y, size_t y_pitch, size_t tokens, void *stream) {
     const Rows xr = {x, x_pitch}, br = {base, base_pitch};
-    if (tokens <= FEW_TOKENS)
+    // A cluster per token costs a token its adapter out of L2 every time, the grouped products three launches: us, cluster | grouped, 2048 -> 2048
+    // unless said: rank 16 (2048 -> 512) 128 tokens 8.6 | 15; rank 32 128 tokens 11 | 16; rank 64 64 tokens 11 | 19, 96 tokens 18 | 19, 128 tokens
+    // 21 | 19; rank 128 (512 -> 2048) 64 tokens 19 | 21, 96 tokens 30 | 21.
+    if (tokens <= 64 || (tokens <= 192 && tokens * ad->rank <= 5120))
         return (ad->type == 0 ? few<float> : ad->type == 1 ? few<__half> : few<__nv_bfloat16>)(tune, ad, xr, slots, br, y, y_pitch, tokens, (cudaStream_t)stream);
     Shape s;
     if (const int rc = make_lists(tune, ad, slots, tokens, (cudaStream_t)stream, s)) return rc;
