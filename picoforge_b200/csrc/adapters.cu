@@ -31,7 +31,7 @@ extern "C" int qw4sh_allow_smem(const void *kernel, size_t smem);
 namespace {
 
 constexpr uint32_t THREADS = 256, TM = 128;                  // tokens per tile: tcgen05's M (shrink) or most N (expand)
-constexpr uint32_t KC = 64, AHEAD = 1, OPS = 1;              // shrink: columns per step, steps that x is fetched ahead, stages of operands
+constexpr uint32_t KC = 64, AHEAD = 1;                       // shrink: columns per step, steps that x is fetched ahead
 constexpr uint32_t TC = 64;                                  // outer: tokens per step
 
 // ---- PTX ------------------------------------------------------------------------------------------------------------------
@@ -77,6 +77,13 @@ __device__ __forceinline__ void tc_load16(uint32_t addr, float (&v)[16]) {
                  : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
                    "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
                  : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_store16(uint32_t addr, const float (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n"
+                 "tcgen05.wait::st.sync.aligned;"
+                 ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+                   "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+                 : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -381,14 +388,15 @@ __global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__r
 
 // ---- accumulators ---------------------------------------------------------------------------------------------------------
 // An accumulator loses up to a bit's weight at every instruction that adds to it (additions in the tensor core truncate), always towards
-// zero, so what counts is how many add to the same one.  Products of the leading planes go to MAINS accumulators in turn, and
+// zero, so what counts is how many add to the same one.  Products of the leading planes go to two accumulators in turn, and
 // the corrections, 2^-8 of them and less, to one of their own (`side`), where their truncations are as much smaller; the sums meet
-// in FP32 when they are read.  With all six products in one accumulator dA of 8192 tokens was 5.9e-6 off, as the plain form in FP32 is
-// 0.9e-6.  Two of the leading planes where that leaves the TMEM columns of three CTAs to an SM.
+// in FP32 when they are read.  Every FLUSH steps they are added to a fourth set of columns, rounded to nearest, and begun anew, so
+// that neither the length of the sum nor how it is cut matters.  Measured with one accumulator for everything: dA of 8192 tokens off by
+// 5.9e-6 of its norm (the plain form in FP32: 0.9e-6); with one for the leading planes and no flush up to 1.8e-6.
+constexpr uint32_t FLUSH = 16;
 template <uint32_t RP> struct Sums {
-    static constexpr uint32_t MAINS = RP <= 32 ? 2 : 1, SIDE = MAINS * RP, NEED = SIDE + RP;
-    static constexpr uint32_t COLS = NEED <= 64 ? 64 : NEED <= 128 ? 128 : 256;                      // TMEM is handed out in powers of two
-    static constexpr uint32_t CTAS = COLS <= 128 ? 3 : 2;    // to an SM
+    static constexpr uint32_t MAINS = 2, SIDE = 2 * RP, TOTAL = 3 * RP, COLS = 4 * RP;
+    static constexpr uint32_t CTAS = RP <= 32 ? 3 : RP == 64 ? 2 : 1;                // to an SM, which has 512 columns
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
@@ -418,16 +426,35 @@ __device__ __forceinline__ void step_mma(uint32_t d, uint32_t d_step, uint32_t s
     for (uint32_t k = 0; k < K16S; k++)
         tc_mma(d + k % MAINS * d_step, a + (k * TA::k16(AMN) >> 4), b + (k * TB::k16(BMN) >> 4), idesc, d_step == 0 || k >= MAINS ? 1 : more);
 }
-// Sixteen columns of a sum that lies in the accumulators of shrink and outer.
-template <uint32_t RP> __device__ __forceinline__ void load_sum(uint32_t addr, float (&v)[16], uint32_t mains = Sums<RP>::MAINS) {
+// Sixteen columns of a sum that lies in the accumulators of shrink and outer: what was added up since the last flush (`mains`: leading accumulators
+// that are in use), and what was before it.
+template <uint32_t RP> __device__ __forceinline__ void load_sum(uint32_t addr, float (&v)[16], uint32_t mains, bool flushed) {
     float u[16];
     tc_load16(addr, v);
+    tc_load16(addr + Sums<RP>::SIDE, u);
 #pragma unroll
-    for (uint32_t m = 1; m <= Sums<RP>::MAINS; m++) {
-        tc_load16(addr + m * RP, u);
+    for (int i = 0; i < 16; i++) v[i] += u[i];
+    if (mains > 1) {
+        tc_load16(addr + RP, u);
 #pragma unroll
-        for (int i = 0; i < 16; i++) v[i] += m == Sums<RP>::MAINS || m < mains ? u[i] : 0.0f;
+        for (int i = 0; i < 16; i++) v[i] += u[i];
     }
+    if (flushed) {
+        tc_load16(addr + Sums<RP>::TOTAL, u);
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] += u[i];
+    }
+}
+// By all warps, between the products of one step and the next: the accumulators to the total.
+template <uint32_t RP> __device__ __forceinline__ void flush(uint32_t tmem, bool again) {
+    const uint32_t warp = threadIdx.x >> 5, lanes = tmem + ((warp & 3) << 21);
+    tc_after();
+    for (uint32_t c = (warp >> 2) * 16; c < RP; c += 32) {
+        float v[16];
+        load_sum<RP>(lanes + c, v, Sums<RP>::MAINS, again);
+        tc_store16(lanes + Sums<RP>::TOTAL + c, v);
+    }
+    tc_before();
 }
 
 // ---- shrink -----------------------------------------------------------------------------------------------------------------
@@ -455,7 +482,7 @@ template <typename W, uint32_t RP> struct ShrinkMap {
     static constexpr uint32_t XU = TM * KC / 4 / THREADS;    // runs of four values of x per thread and step
     static constexpr uint32_t W_UNIT = THREADS * 4 * sizeof(W), SLOT = XU * THREADS * 16 + Run::UNITS * W_UNIT;
     static constexpr uint32_t OPERANDS = X::BYTES + Run::BYTES;
-    static constexpr uint32_t ORDER = 64, STAGE = ORDER + TM * 4, RING = STAGE + OPS * OPERANDS, END = RING + AHEAD * SLOT;
+    static constexpr uint32_t ORDER = 64, STAGE = ORDER + TM * 4, RING = STAGE + OPERANDS, END = RING + AHEAD * SLOT;
     static constexpr uint32_t PITCH = RP + 4;                // floats per row of the exchanged accumulators
     static constexpr uint32_t ACC_END = STAGE + TM * PITCH * 4, TOTAL = END > ACC_END ? END : ACC_END;
 };
@@ -463,7 +490,7 @@ template <typename W, uint32_t RP> struct ShrinkMap {
 // Values come in by asynchronous copies, AHEAD steps before they are cut, each thread's own into places of its own: no barrier, no register and no line
 // of L1 holds them meanwhile (through registers an SM had half as many bytes under way).
 template <typename W, uint32_t RP>
-__global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel(const __grid_constant__ ShrinkArgs<W> a) {
+__global__ void __launch_bounds__(THREADS, RP <= 64 ? 2 : 1) adapter_shrink_kernel(const __grid_constant__ ShrinkArgs<W> a) {
     namespace cg = cooperative_groups;
     using M = ShrinkMap<W, RP>;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -526,9 +553,10 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
     for (uint32_t s = 0; s < AHEAD; s++) copy(s);
     const uint32_t idesc = idesc_of(TM, RP, false, !m.wide);
     for (uint32_t s = 0; s < steps; s++) {
-        const uint32_t c0 = c_first + s * KC, slot = s % AHEAD * M::SLOT, at = base + M::STAGE + s % OPS * M::OPERANDS, wat = at + M::X::BYTES, bar = base + 8 * (s % OPS);
+        const uint32_t c0 = c_first + s * KC, slot = s % AHEAD * M::SLOT, at = base + M::STAGE, wat = at + M::X::BYTES;
         copies_wait<AHEAD - 1>();
-        if (s >= OPS) bar_wait(bar, (s / OPS - 1) & 1, a.status);
+        if (s) bar_wait(base, (s - 1) & 1, a.status);
+        if (s && s % FLUSH == 0) flush<RP>(tmem, s > FLUSH);
 #pragma unroll
         for (uint32_t i = 0; i < XU; i++) {
             Four<float> xv;
@@ -543,21 +571,21 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_shrink_kernel
         if (warp == 0) {
             tc_after();
             const uint32_t leader = elect();                 // the thread whose products the commit answers for
-            if (m.wide) step_mma<typename M::X, typename M::Run::Wide, 3, M::Run::PLANES, false, false, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, at, wat, idesc, s == 0, leader);
-            else step_mma<typename M::X, typename M::Run::Tall, 3, M::Run::PLANES, false, true, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, at, wat, idesc, s == 0, leader);
-            if (leader) tc_commit(bar);
+            if (m.wide) step_mma<typename M::X, typename M::Run::Wide, 3, M::Run::PLANES, false, false, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, at, wat, idesc, s % FLUSH == 0, leader);
+            else step_mma<typename M::X, typename M::Run::Tall, 3, M::Run::PLANES, false, true, Sums<RP>::MAINS, KC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, at, wat, idesc, s % FLUSH == 0, leader);
+            if (leader) tc_commit(base);
             __syncwarp();
         }
     }
     copies_wait<0>();
-    if (steps) bar_wait(base + 8 * ((steps - 1) % OPS), ((steps - 1) / OPS) & 1, a.status);
+    if (steps) bar_wait(base, (steps - 1) & 1, a.status);
     tc_after();
     grid_go();                                               // not before: CTAs of the next launch would crowd onto the SMs that are done first
     // accumulators to shared memory, summed over the cluster's CTAs in their order, scaled, cut and stored
     float *acc = (float *)(smem + M::STAGE);
     for (uint32_t c = (warp >> 2) * 16; c < RP; c += 32) {
         float v[16];
-        load_sum<RP>(tmem + ((warp & 3) << 21) + c, v);
+        load_sum<RP>(tmem + ((warp & 3) << 21) + c, v, Sums<RP>::MAINS, steps > FLUSH);
         float *row = acc + ((warp & 3) * 32 + lane) * M::PITCH + c;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) *(float4 *)(row + i) = steps ? make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_float4(0, 0, 0, 0);
@@ -783,6 +811,7 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     for (uint32_t s = 0; s < steps; s++) {
         const uint32_t t0 = from + s * TC;
         if (s) bar_wait(base, (s - 1) & 1, a.status);
+        if (s && s % FLUSH == 0) flush<RP>(tmem, s > FLUSH);
         const uint32_t rows16 = uniform((min(to - t0, TC) + 15) & ~15u);
         if (tid == 0) copy_rank<TC, RP>(base + M::H_AT, job.planes, a.plane, begin + t0, rows16, base + 8);       // out of L2, while x is cut
 #pragma unroll
@@ -795,11 +824,11 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
             __syncwarp();
             const uint32_t leader = elect();
             if (rows16 == TC)
-                step_mma<typename M::X, typename M::H, 3, 3, true, true, Sums<RP>::MAINS, TC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::H_AT, idesc, s == 0, leader);
+                step_mma<typename M::X, typename M::H, 3, 3, true, true, Sums<RP>::MAINS, TC / 16>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE, base + M::H_AT, idesc, s % FLUSH == 0, leader);
             else                                             // the last tokens; into one of the leading accumulators alone, the others as they are
                 for (uint32_t k = 0; k < rows16 / 16; k++)
                     step_mma<typename M::X, typename M::H, 3, 3, true, true, 1, 1>(tmem, RP, tmem + Sums<RP>::SIDE, base + M::STAGE + k * M::X::k16(true),
-                                                                                    base + M::H_AT + k * M::H::k16(true), idesc, s == 0 && k == 0, leader);
+                                                                                    base + M::H_AT + k * M::H::k16(true), idesc, s % FLUSH == 0 && k == 0, leader);
             if (leader) tc_commit(base);
             __syncwarp();
         }
@@ -808,10 +837,12 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
     if (steps) bar_wait(base, (steps - 1) & 1, a.status);
     tc_after();
     grid_go();
+    // the last tokens alone, if no whole step came before them since the last flush, are in one leading accumulator
+    const uint32_t mains = steps && to - from - (steps - 1) / FLUSH * (FLUSH * TC) + 15 < TC ? 1 : Sums<RP>::MAINS;
     float *acc = (float *)(smem + M::STAGE);
     for (uint32_t c = (warp >> 2) * 16; c < RP; c += 32) {
         float v[16];
-        load_sum<RP>(tmem + ((warp & 3) << 21) + c, v, to - from + 15 < TC ? 1 : Sums<RP>::MAINS);
+        load_sum<RP>(tmem + ((warp & 3) << 21) + c, v, mains, steps > FLUSH);
 #pragma unroll
         for (uint32_t i = 0; i < 16; i++) acc[(c + i) * M::PITCH + (warp & 3) * 32 + lane] = steps ? v[i] : 0.0f;
     }

@@ -1,7 +1,7 @@
 """Low-rank adapters beside a projection and their gradients against the formulas in 64 bits.
 
-Bounds.  u = 2^-24 is half a step of FP32.  x enters as a sum of three bf16 values, each off by at most 2^-9 of what is left, so off by
-2^-27 |x| in all, and F32 adapters likewise; what is left of the products beyond the second order is below 2^-24 of them.  A sum of n terms in FP32 whose additions may
+Bounds.  u = 2^-24 is half a step of FP32.  x enters as a sum of three bf16 values that is x, and F32 adapters likewise; what is left
+out of their products, beyond the second order, is below 2^-23 of them.  A sum of n terms in FP32 whose additions may
 truncate (tensor cores) is off by at most 2 n u times the sum of the terms' sizes.  So every value is held to 2 u (n + 16) S, S the same formula on absolute
 values and n the terms of both sums (`worst`), and all of them together, where errors of random sign add up like sqrt(n), to 4 u sqrt(n + 16) relative to
 the norm of what the adapters give (`spread`), plus u for the one addition of base."""
@@ -140,6 +140,12 @@ def test_where_the_tokens_of_a_slot_lie(api, t, k, n, r, s, pattern):
     y, dx, da, db = check(api, c)
     if pattern == "none":
         assert torch.equal(y, c.by) and torch.equal(dx, c.bx) and not da.any() and not db.any()
+
+
+@pytest.mark.parametrize("t,k,n,r", [(8200, 8192, 64, 24), (1044, 19200, 19200, 16), (1030, 19200, 19200, 64), (3000, 12000, 130, 128)])
+def test_sums_longer_than_an_accumulator_takes(api, t, k, n, r):
+    """Runs of more than 1024 columns or tokens to a CTA: accumulators are put by and begun anew; the last of them may have a few tokens alone."""
+    check(api, Case(t, k, n, r, 1, torch.bfloat16, "one"))
 
 
 @pytest.mark.parametrize("pad", [1, 2, 4])
