@@ -590,10 +590,12 @@ __global__ void __launch_bounds__(THREADS, RP <= 64 ? 2 : 1) adapter_shrink_kern
 #pragma unroll
         for (int i = 0; i < 16; i += 4) *(float4 *)(row + i) = steps ? make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_float4(0, 0, 0, 0);
     }
+    // TMEM goes back before the CTAs wait for one another: two clusters that each held columns which a CTA of the other was waiting for
+    // would wait for good
     tc_before();
+    __syncthreads();
+    if (warp == 0) { tc_after(); tc_free(tmem, Sums<RP>::COLS); }
     cluster.sync();
-    tc_after();
-    if (warp == 0) tc_free(tmem, Sums<RP>::COLS);
     const float scale = a.scale ? a.scale[t.slot] : 1.0f;
     const uint32_t rows = TM / parts, rows16 = (t.rows + 15) & ~15u;
     for (uint32_t u = tid; u < rows * (RP / 4); u += THREADS) {
@@ -846,10 +848,12 @@ __global__ void __launch_bounds__(THREADS, Sums<RP>::CTAS) adapter_outer_kernel(
 #pragma unroll
         for (uint32_t i = 0; i < 16; i++) acc[(c + i) * M::PITCH + (warp & 3) * 32 + lane] = steps ? v[i] : 0.0f;
     }
+    // TMEM goes back before the CTAs wait for one another: two clusters that each held columns which a CTA of the other was waiting for
+    // would wait for good
     tc_before();
+    __syncthreads();
+    if (warp == 0) { tc_after(); tc_free(tmem, Sums<RP>::COLS); }
     cluster.sync();
-    tc_after();
-    if (warp == 0) tc_free(tmem, Sums<RP>::COLS);
     for (uint32_t u = part * THREADS + tid; u < RP * 32; u += parts * THREADS) {
         // neighbouring threads: neighbouring columns of dA, neighbouring r of dB
         const uint32_t r = sc == 1 ? u / 32 : u % RP, c = (sc == 1 ? u % 32 : u / RP) * 4;
@@ -943,6 +947,7 @@ __global__ void __launch_bounds__(THREADS, 4) adapter_few_kernel(const __grid_co
     }
     const W *A = a.a + (uint64_t)s * R * a.k, *B = a.b + (uint64_t)s * R * a.n;
     const float *x = a.x + t * a.x_pitch;
+    cluster.barrier_arrive();                                // whoever writes to another CTA's shared memory has to know that it has begun
 
     // rows of B: `span` lanes to a row, so that a load of a warp is one run of memory
     uint32_t span = 1;
@@ -984,12 +989,14 @@ __global__ void __launch_bounds__(THREADS, 4) adapter_few_kernel(const __grid_co
         for (uint32_t j = 0; j < RANKS; j++)
 #pragma unroll
             for (int o = 16; o; o >>= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
+        if (r0 == warp) cluster.barrier_wait();
         if (lane < FEW_CTAS) {
             float *to = cluster.map_shared_rank(&partial[part][0], lane);
 #pragma unroll
             for (uint32_t j = 0; j < RANKS; j++) if (r0 + 8 * j < R) to[r0 + 8 * j] = sum[j];
         }
     }
+    if (warp >= R) cluster.barrier_wait();                   // a warp without an r
     cluster.sync();
     if (tid < R) {
         float sum = 0;
