@@ -21,8 +21,16 @@ constexpr uint32_t THREADS = 256;
 constexpr float UNIT = 1099511627776.0f;          // 2^40: probability sums meet as 64-bit integers, whose sum has no order
 
 __device__ __forceinline__ float warp_max(float v) {
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    float m;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+}
+// exp(v - m) as 2^((v - m) log2 e): the difference and the product are rounded once each and the instruction is off by 2^-22 at most; -inf gives
+// zero, and what has no softmax (a NaN, a +inf, nothing but -inf) a NaN.
+__device__ __forceinline__ float exp_of(float v, float m) {
+    float e;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"((v - m) * 1.4426950408889634f));
+    return e;
 }
 __device__ __forceinline__ float warp_sum(float v) {
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -63,7 +71,7 @@ template <int PER, bool VEC> struct Row {
         m = warp_max(m);
         float s = 0;
 #pragma unroll
-        for (int i = 0; i < PER; i++) { v[i] = expf(v[i] - m); s += v[i]; }
+        for (int i = 0; i < PER; i++) { v[i] = exp_of(v[i], m); s += v[i]; }
         return warp_sum(s);
     }
 };
@@ -248,11 +256,11 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(uint32_t E, u
             const float inv = 1.0f / s;
             float sum = 0;
 #pragma unroll
-            for (int i = 0; i < PER; i++) { row.v[i] *= inv; sum = fmaf(row.v[i], f[i], sum); }
-            shared = warp_sum(sum);
+            for (int i = 0; i < PER; i++) sum = fmaf(row.v[i], f[i], sum);
+            shared = warp_sum(sum) * inv;
             if (dw) {
                 if (chosen && my_id >= E) atomicOr(status, QW4SH_ERR_BOUNDS);
-                p_mine = in ? expf(zc - m) * inv : 0.0f;
+                p_mine = in ? exp_of(zc, m) * inv : 0.0f;
                 if (norm) {
                     const float top = warp_max(in ? zc : -CUDART_INF_F), w = in ? expf(zc - top) : 0.0f;
                     const float weight = w / warp_sum(w);
@@ -265,8 +273,9 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(uint32_t E, u
                 }
                 same = __match_any_sync(0xffffffffu, in ? my_id : 0x80000000u | lane);
             }
+            const float off = shared * inv;
 #pragma unroll
-            for (int i = 0; i < PER; i++) values[i] = row.v[i] * (f[i] - shared);
+            for (int i = 0; i < PER; i++) values[i] = row.v[i] * fmaf(f[i], inv, -off);
         } else {
 #pragma unroll
             for (int i = 0; i < PER; i++) values[i] = 0;
