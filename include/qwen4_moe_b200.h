@@ -583,8 +583,7 @@ typedef struct {
 /* y[t] = base[t] + scale_s B_s (A_s x[t]) with s = slots_dev[t]; y[t] = base[t] where that is QW4CU_NO_ADAPTER (or
  * out of range).  base NULL: zero; base may be y itself (same pitch), otherwise y must not overlap what is read.
  * Pitches are bytes between rows.  x [tokens, k], base and y [tokens, n].  Tokens of a slot may lie anywhere in the
- * batch.  Products of F16 and BF16 adapters are exact and summed in FP32; x, and F32 adapters, enter the tensor
- * cores as a sum of three bf16 values (24 bits). */
+ * batch.  Values enter the products with all their bits and are summed in FP32 (of products of two FP32 values 2^-21 at most is left out). */
 Qwen4Status qw4cu_adapter_forward_device(const QW4CuAdapters *adapters, const float *x_dev, size_t x_pitch, const uint32_t *slots_dev,
                                          const float *base_dev, size_t base_pitch, float *y_dev, size_t y_pitch, size_t tokens,
                                          QW4CuTuneWork *work, Qwen4Error *err);

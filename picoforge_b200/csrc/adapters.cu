@@ -10,7 +10,7 @@
 //   outer   [tokens of a slot] -> [128 columns, rank]         dA and dB: contracts the tokens, cut over a cluster's CTAs
 // All on tcgen05 with FP32 accumulators in TMEM.  An FP32 value enters as three bf16 values, its 24 bits cut in three (each
 // a truncation, so their sum is the value exactly); F16 adapters as two, BF16 ones as they are.  Products of planes i and j are formed for
-// i + j <= 2; what is left out is below 2^-24 of a product.
+// i + j <= 2; what is left out is below 2^-21 of a product of two FP32 values, 2^-25 on average.
 //
 // Operands are written to shared memory by the CTA's threads, which cut them on the way, as 8 x 16-byte core matrices without
 // swizzle: [8 columns][8 rows][16 bytes], so that rows of the source can be the rows of either major-ness.  Column groups
@@ -25,7 +25,6 @@
 #include "cuda_shim.h"
 
 extern "C" int qw4sh_note_launch(const char *name);
-extern "C" int qw4sh_fail_text(const char *text);
 extern "C" int qw4sh_allow_smem(const void *kernel, size_t smem);
 
 namespace {

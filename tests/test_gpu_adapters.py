@@ -1,7 +1,7 @@
 """Low-rank adapters beside a projection and their gradients against the formulas in 64 bits.
 
 Bounds.  u = 2^-24 is half a step of FP32.  x enters as a sum of three bf16 values that is x, and F32 adapters likewise; what is left
-out of their products, beyond the second order, is below 2^-23 of them.  A sum of n terms in FP32 whose additions may
+out of their products, beyond the second order, is below 2^-21 of them (so inside the sixteen of the bound below).  A sum of n terms in FP32 whose additions may
 truncate (tensor cores) is off by at most 2 n u times the sum of the terms' sizes.  So every value is held to 2 u (n + 16) S, S the same formula on absolute
 values and n the terms of both sums (`worst`), and all of them together, where errors of random sign add up like sqrt(n), to 4 u sqrt(n + 16) relative to
 the norm of what the adapters give (`spread`), plus u for the one addition of base."""
