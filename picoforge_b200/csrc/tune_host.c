@@ -11,7 +11,7 @@ struct QW4CuTuneWork {
     QW4CuTuneLimits limits;
     int device;
     bool failed;
-    size_t device_bytes;
+    size_t device_bytes, clear_bytes;     /* what has to be zero between launches lies in front */
     unsigned char *block;                 /* one device allocation carved into d.* */
     uint32_t status_host[4];
     QW4ShTune d;
@@ -60,6 +60,7 @@ Qwen4Status qw4cu_tune_work_create(const QW4CuTuneLimits *limits, QW4CuTuneWork 
     w->device = qw4sh_current_device();
     size_t at = 0;
     const size_t status = take(&at, 16), sums = take(&at, (size_t)l.experts * 8), counts = take(&at, ((size_t)l.experts + 2) * 4);
+    w->clear_bytes = at;
     const bool adapters = l.slots != 0;
     const size_t places = adapters ? qw4sh_adapter_rows(l.tokens, l.slots) : 0;
     const size_t order = take(&at, places * 4), offsets = take(&at, adapters ? ((size_t)l.slots + 1) * 8 : 0);
@@ -84,7 +85,7 @@ Qwen4Status qw4cu_tune_work_create(const QW4CuTuneLimits *limits, QW4CuTuneWork 
     w->d.n_tiles = (uint32_t *)(w->block + n_tiles);
     w->d.h = w->block + h;
     w->d.g = w->block + g;
-    if (qw4sh_memset_async(w->block, 0, at, stream) || status_clear(w, stream) || qw4sh_stream_sync(stream)) {
+    if (qw4sh_memset_async(w->block, 0, w->clear_bytes, stream) || status_clear(w, stream) || qw4sh_stream_sync(stream)) {
         const Qwen4Status st = cuda_answer(err, "workspace clear");
         qw4cu_tune_work_destroy(w);
         return st;
@@ -127,7 +128,7 @@ Qwen4Status qw4cu_tune_work_reset(QW4CuTuneWork *w, Qwen4Error *err) {
     void *stream;
     const Qwen4Status st = stream_of(w, &stream, err);
     if (st != QW4_OK) return st;
-    if (qw4sh_memset_async(w->block, 0, w->device_bytes, stream) || status_clear(w, stream) || qw4sh_stream_sync(stream))
+    if (qw4sh_memset_async(w->block, 0, w->clear_bytes, stream) || status_clear(w, stream) || qw4sh_stream_sync(stream))
         return cuda_answer(err, "workspace clear");
     w->failed = false;
     return answer(err, QW4_OK, "");
