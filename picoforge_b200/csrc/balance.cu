@@ -25,11 +25,11 @@ __device__ __forceinline__ float warp_max(float v) {
     asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
     return m;
 }
-// exp(v - m) as 2^((v - m) log2 e): the difference and the product are rounded once each and the instruction is off by 2^-22 at most; -inf gives
-// zero, and what has no softmax (a NaN, a +inf, nothing but -inf) a NaN.
+// exp(v - m) as 2^((v - m) log2 e): the difference and the product are rounded once each and the instruction is off by 2^-22 at most (results below
+// 2^-126 are zero: the form that keeps them takes four instructions, and these kernels are bound by them); -inf gives zero, and what has no softmax (a NaN, a +inf, nothing but -inf) a NaN.
 __device__ __forceinline__ float exp_of(float v, float m) {
     float e;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"((v - m) * 1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v - m) * 1.4426950408889634f));
     return e;
 }
 __device__ __forceinline__ float warp_sum(float v) {

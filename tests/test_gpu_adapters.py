@@ -323,8 +323,9 @@ def test_captured_into_a_graph_and_replayed_on_other_values(api):
                 assert torch.equal(p, q)
 
 
-def test_two_workspaces_on_two_streams_at_once(api):
-    cases = [Case(700, 512, 512, 16, 3, torch.bfloat16, seed=i) for i in (1, 2)]
+@pytest.mark.parametrize("t,r", [(700, 16), (2500, 64), (1500, 128)])
+def test_two_workspaces_on_two_streams_at_once(api, t, r):
+    cases = [Case(t, 512, 512, r, 3, torch.bfloat16, seed=i) for i in (1, 2)]
     works = [c.work(api) for c in cases]
     want = [(forward(w, c), *backward(w, c)) for w, c in zip(works, cases)]
     streams = [torch.cuda.Stream() for _ in cases]
