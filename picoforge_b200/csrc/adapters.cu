@@ -1095,12 +1095,13 @@ uint32_t cluster_of(uint64_t items, uint64_t length, uint32_t least, uint32_t ct
 }
 
 template <typename W, uint32_t RP>
-int shrink(const ShrinkJob<W> *jobs, uint32_t n, const Shape &s) {
+int shrink(const ShrinkJob<W> *jobs, uint32_t all, uint32_t n, const Shape &s) {
+    // cut as for all the jobs that there may be: the bits of one do not depend on whether the other was asked for
     ShrinkArgs<W> a = {};
     uint64_t width = 0;
-    for (uint32_t i = 0; i < n; i++) { a.job[i] = jobs[i]; if (jobs[i].w.width > width) width = jobs[i].w.width; }
+    for (uint32_t i = 0; i < all; i++) { a.job[i] = jobs[i]; if (jobs[i].w.width > width) width = jobs[i].w.width; }
     a.lists = s.lists; a.scale = s.scale; a.plane = s.plane; a.slots = s.S; a.status = s.status;
-    const uint32_t c = cluster_of((uint64_t)(s.T + TM - 1) / TM * n, width, 128, 2 * SMS, most_ctas((const void *)adapter_shrink_kernel<W, RP>, ShrinkMap<W, RP>::TOTAL));
+    const uint32_t c = cluster_of((uint64_t)(s.T + TM - 1) / TM * all, width, 128, 2 * SMS, most_ctas((const void *)adapter_shrink_kernel<W, RP>, ShrinkMap<W, RP>::TOTAL));
     return launch(adapter_shrink_kernel<W, RP>, "adapter_shrink_kernel", dim3(c, s.tiles, n), THREADS, ShrinkMap<W, RP>::TOTAL, c, true, s.stream, a);
 }
 template <typename W, uint32_t RP>
@@ -1137,7 +1138,7 @@ int few(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, const uint32_t *
 template <typename W, uint32_t RP>
 int forward(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, Rows base, float *y, size_t y_pitch, const Shape &s) {
     const ShrinkJob<W> job = {mat_a<W>(ad), x.p, x.pitch, runs(x, s.T), (__nv_bfloat16 *)tune->h};
-    if (const int rc = shrink<W, RP>(&job, 1, s)) return rc;
+    if (const int rc = shrink<W, RP>(&job, 1, 1, s)) return rc;
     return expand<W, RP>(mat_b<W>(ad), job.planes, base.p, base.pitch, y, y_pitch, s);
 }
 template <typename W, uint32_t RP>
@@ -1145,7 +1146,7 @@ int backward(const QW4ShTune *tune, const QW4CuAdapters *ad, Rows x, Rows dy, Ro
     const ShrinkJob<W> jobs[2] = {{mat_b<W>(ad), dy.p, dy.pitch, runs(dy, s.T), (__nv_bfloat16 *)tune->g},
                                   {mat_a<W>(ad), x.p, x.pitch, runs(x, s.T), (__nv_bfloat16 *)tune->h}};
     int rc;
-    if ((rc = shrink<W, RP>(jobs, da ? 2 : 1, s))) return rc;
+    if ((rc = shrink<W, RP>(jobs, 2, da ? 2 : 1, s))) return rc;
     const OuterJob outers[2] = {{x.p, x.pitch, (uint32_t)ad->k, jobs[1].x_fours, jobs[0].planes, da, (uint32_t)ad->k, 1, (uint32_t)((ad->k + 127) / 128)},
                                 {dy.p, dy.pitch, (uint32_t)ad->n, jobs[0].x_fours, jobs[1].planes, db, 1, ad->rank, (uint32_t)((ad->n + 127) / 128)}};
     // dA and dB behind shrink, which has just read what they read

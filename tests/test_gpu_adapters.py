@@ -185,6 +185,33 @@ def test_base_absent_in_place_or_elsewhere(api, t):
     assert not alone[c.slot < 0].any()
 
 
+@pytest.mark.parametrize("t", [2, 90, 600])
+def test_rows_of_different_pitch_and_dx_in_place(api, t):
+    c = Case(t, 256, 192, 16, 4, torch.float16)
+    with c.work(api) as work:
+        want, (dx, da, db) = forward(work, c), backward(work, c)
+        wide_base, wide_y = torch.zeros(t, 192 + 8, device="cuda"), torch.zeros(t, 192 + 12, device="cuda")
+        wide_base[:, :192] = c.by
+        forward(work, c, wide_y[:, :192], base=wide_base[:, :192])
+        place = c.bx.clone()
+        work.adapter_backward(c.view(), c.x.data_ptr(), c.slot.data_ptr(), c.dy.data_ptr(), place.data_ptr(), place.data_ptr(), None, None, t)
+        work.sync()
+    assert torch.equal(wide_y[:, :192], want) and not wide_y[:, 192:].any() and torch.equal(place, dx)
+
+
+def test_a_smaller_call_on_a_larger_workspace(api):
+    """The scratch is laid out by the call, not by the limits: other slots, ranks and token counts in turn, stale contents behind."""
+    with tuning.TuneWork(api, tokens=3000, slots=40, rank=128) as work:
+        for t, k, n, r, slots in ((3000, 128, 64, 128, 40), (100, 64, 96, 8, 3), (700, 96, 64, 33, 7), (1, 64, 64, 16, 1), (2999, 64, 128, 17, 40)):
+            c = Case(t, k, n, r, slots, torch.bfloat16)
+            y, (dx, da, db) = forward(work, c), backward(work, c)
+            work.sync()
+            with c.work(api) as own:
+                for p, q in zip((y, dx, da, db), (forward(own, c), *backward(own, c))):
+                    assert torch.equal(p, q)
+                own.sync()
+
+
 @pytest.mark.parametrize("t", [3, 64, 300])
 def test_parts_of_the_gradient_and_the_same_bits_twice(api, t):
     c = Case(t, 256, 512, 16, 3, torch.bfloat16)
@@ -201,7 +228,7 @@ def test_parts_of_the_gradient_and_the_same_bits_twice(api, t):
 
 
 def test_scale_absent(api):
-    for t in (3, 100):
+    for t in (3, 100, 400):
         c = Case(t, 64, 64, 8, 2, torch.float32)
         c.scale = torch.ones(2, device="cuda")
         with c.work(api) as work:
@@ -214,7 +241,7 @@ def test_scale_absent(api):
         assert torch.equal(y, z)
 
 
-@pytest.mark.parametrize("t", [0, 4, 80])
+@pytest.mark.parametrize("t", [0, 4, 80, 300])
 def test_slots_out_of_range_and_no_tokens(api, t):
     c = Case(t, 64, 64, 8, 2, torch.bfloat16)
     with c.work(api) as work:
@@ -275,9 +302,10 @@ def test_large_and_small_values(api):
             close(y, want, sizes, c.k + c.r)
 
 
-def test_offsets_beyond_32_bits(api):
-    """Rows of x and y that lie more than 2^31 floats apart from the first."""
-    t, step = 40, 1 << 26
+@pytest.mark.parametrize("t,step", [(40, 1 << 26), (300, 1 << 24)])
+def test_offsets_beyond_32_bits(api, t, step):
+    """Rows of x and y that lie more than 2^31 floats (and 2^32) apart from the first."""
+    torch.cuda.empty_cache()
     c = Case(t, 256, 128, 8, 2, torch.bfloat16)
     x = torch.empty((t - 1) * step + 256, device="cuda").as_strided((t, 256), (step, 1))
     x.copy_(c.x)
