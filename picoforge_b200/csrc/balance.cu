@@ -20,9 +20,10 @@ namespace {
 constexpr uint32_t THREADS = 256;
 constexpr float UNIT = 1099511627776.0f;          // 2^40: probability sums meet as 64-bit integers, whose sum has no order
 
+// By all lanes of a warp together: volatile, or the compiler may move it to where its result is used, which not every lane reaches.
 __device__ __forceinline__ float warp_max(float v) {
     float m;
-    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
     return m;
 }
 // exp(v - m) as 2^((v - m) log2 e): the difference and the product are rounded once each and the instruction is off by 2^-22 at most (results below
@@ -262,7 +263,8 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(uint32_t E, u
                 if (chosen && my_id >= E) atomicOr(status, QW4SH_ERR_BOUNDS);
                 p_mine = in ? exp_of(zc, m) * inv : 0.0f;
                 if (norm) {
-                    const float top = warp_max(in ? zc : -CUDART_INF_F), w = in ? expf(zc - top) : 0.0f;
+                    const float top = warp_max(in ? zc : -CUDART_INF_F);
+                    const float w = in ? expf(zc - top) : 0.0f;
                     const float weight = w / warp_sum(w);
                     const float mean = warp_sum(in ? weight * my_d : 0.0f);
                     total = in ? weight * (my_d - mean) : 0.0f;

@@ -47,3 +47,11 @@ def test_barriers_are_fenced_before_copies_and_products_use_them(source):
         if inits:
             meet = body.find("__syncthreads()", inits[-1])
             assert meet > 0 and re.search(r"fence\.(mbarrier_init|proxy\.async)", body[inits[-1]:meet]), body[inits[-1]:inits[-1] + 300]
+
+
+@pytest.mark.parametrize("source", SOURCES, ids=lambda p: p.name)
+def test_collectives_stay_where_they_are_written(source):
+    """An asm statement that is not volatile may move to where its result is used, which only some of the lanes may reach; one in
+    which all lanes of a warp have to take part then never ends."""
+    for m in re.finditer(r"\basm\s*\(\s*\"[^\"]*\b(redux|elect|vote|shfl|match|bar|barrier|activemask)\.", without_comments(source.read_text())):
+        pytest.fail(f"{source.name}: collective in an asm that is not volatile: {m.group(0)}")
