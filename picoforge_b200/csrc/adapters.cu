@@ -88,6 +88,7 @@ __device__ __forceinline__ void tc_store16(uint32_t addr, const float (&v)[16]) 
                  : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// As in balance.cu: nothing that the launch ahead wrote is read before the wait, or through a __restrict__ pointer to const.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -294,7 +295,7 @@ template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
 // multiple of sixteen on; tiles of up to 128 tokens of one slot.  One CTA: every warp counts a run of tokens, then places it.
 struct ATile { uint32_t slot, first, rows, pad; };
 
-__global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *__restrict__ ids, uint32_t T, uint32_t S, uint32_t *__restrict__ order,
+__global__ void __launch_bounds__(1024) adapter_lists_kernel(const uint32_t *ids, uint32_t T, uint32_t S, uint32_t *__restrict__ order,
                                                              uint32_t *__restrict__ offsets /* [groups][start, tokens] */, ATile *__restrict__ tiles,
                                                              uint32_t *__restrict__ n_tiles, uint32_t *status) {
     extern __shared__ uint32_t counts[];                     // [warps][S + 1], then where the groups start [S + 1]

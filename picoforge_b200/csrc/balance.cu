@@ -38,6 +38,8 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Kernels here may begin before the launch ahead of them has ended: before the wait they read nothing, and what they read after it is no
+// __restrict__ pointer to const, whose loads the compiler would be free to put before it.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // A row that has no softmax is noted with its number (the lowest is kept).
@@ -114,8 +116,8 @@ __device__ __forceinline__ void balance_finish(uint32_t E, const QW4ShTune &tune
 // A warp to a row, the next row on its way while one is summed; every lane adds up its columns in registers over the rows of its warp,
 // the warps of a CTA add theirs in shared memory, the CTAs as integers.
 template <int PER, bool VEC>
-__global__ void __launch_bounds__(THREADS) balance_forward_kernel(uint32_t E, uint32_t K, const float *__restrict__ logits, uint64_t pitch,
-                                                                  const uint32_t *__restrict__ ids, const uint8_t *__restrict__ mask, uint32_t T,
+__global__ void __launch_bounds__(THREADS) balance_forward_kernel(uint32_t E, uint32_t K, const float *logits, uint64_t pitch,
+                                                                  const uint32_t *ids, const uint8_t *mask, uint32_t T,
                                                                   const __grid_constant__ QW4ShTune tune, uint32_t *__restrict__ counts,
                                                                   float *__restrict__ prob_sums, float *__restrict__ loss) {
     constexpr uint32_t WARPS = THREADS / 32, COLS = 32 * PER;
@@ -174,8 +176,8 @@ __global__ void __launch_bounds__(THREADS) balance_forward_kernel(uint32_t E, ui
 
 // More experts than fit a warp's registers: a warp to a row, three passes over it (the later ones out of L1), every probability
 // added to the CTA's sums as an integer.
-__global__ void __launch_bounds__(THREADS) balance_forward_wide_kernel(uint32_t E, uint32_t K, const float *__restrict__ logits, uint64_t pitch,
-                                                                       const uint32_t *__restrict__ ids, const uint8_t *__restrict__ mask, uint32_t T,
+__global__ void __launch_bounds__(THREADS) balance_forward_wide_kernel(uint32_t E, uint32_t K, const float *logits, uint64_t pitch,
+                                                                       const uint32_t *ids, const uint8_t *mask, uint32_t T,
                                                                        const __grid_constant__ QW4ShTune tune, uint32_t *__restrict__ counts,
                                                                        float *__restrict__ prob_sums, float *__restrict__ loss) {
     extern __shared__ uint32_t shared_words[];               // [E] counts, [E] sums as 64-bit integers
@@ -215,9 +217,9 @@ __global__ void __launch_bounds__(THREADS) balance_forward_wide_kernel(uint32_t 
 
 // A warp to a row.  The share of the route weights is worked out by a lane per chosen expert and laid over the row behind the rest.
 template <int PER, bool VEC>
-__global__ void __launch_bounds__(THREADS) balance_backward_kernel(uint32_t E, uint32_t K, int norm, const float *__restrict__ logits, uint64_t pitch,
-                                                                   const uint32_t *__restrict__ ids, const uint8_t *__restrict__ mask, uint32_t T,
-                                                                   const uint32_t *__restrict__ counts, float loss_grad, const float *__restrict__ dw,
+__global__ void __launch_bounds__(THREADS) balance_backward_kernel(uint32_t E, uint32_t K, int norm, const float *logits, uint64_t pitch,
+                                                                   const uint32_t *ids, const uint8_t *mask, uint32_t T,
+                                                                   const uint32_t *counts, float loss_grad, const float *dw,
                                                                    float *__restrict__ grad, uint64_t gpitch, uint32_t *status) {
     constexpr uint32_t WARPS = THREADS / 32;
     using R = Row<PER, VEC>;
@@ -246,7 +248,8 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(uint32_t E, u
         const float my_d = d;
         float *out = grad + t * gpitch;
         const bool in = chosen && now && my_id < E;
-        if (in) zc = logits[t * pitch + my_id];
+        float f_mine = 0;
+        if (in) { zc = logits[t * pitch + my_id]; f_mine = (float)counts[my_id] * scale; }
         there = fetch(t + step);
         float values[PER], total = 0, shared = 0, p_mine = 0;       // total: the route weights' share
         uint32_t same = 0;
@@ -299,15 +302,15 @@ __global__ void __launch_bounds__(THREADS) balance_backward_kernel(uint32_t E, u
                 total = all;
             }
             __syncwarp();
-            if (in) out[my_id] = p_mine * ((float)counts[my_id] * scale - shared) + total;
+            if (in) out[my_id] = p_mine * (f_mine - shared) + total;
         }
     }
 }
 
 // More experts than fit a warp's registers, or more chosen ones than lanes.
-__global__ void __launch_bounds__(THREADS) balance_backward_wide_kernel(uint32_t E, uint32_t K, int norm, const float *__restrict__ logits, uint64_t pitch,
-                                                                        const uint32_t *__restrict__ ids, const uint8_t *__restrict__ mask, uint32_t T,
-                                                                        const uint32_t *__restrict__ counts, float loss_grad, const float *__restrict__ dw,
+__global__ void __launch_bounds__(THREADS) balance_backward_wide_kernel(uint32_t E, uint32_t K, int norm, const float *logits, uint64_t pitch,
+                                                                        const uint32_t *ids, const uint8_t *mask, uint32_t T,
+                                                                        const uint32_t *counts, float loss_grad, const float *dw,
                                                                         float *__restrict__ grad, uint64_t gpitch, uint32_t *status) {
     const uint32_t lane = threadIdx.x & 31, t = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
     grid_wait();

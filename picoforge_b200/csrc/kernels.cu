@@ -627,7 +627,8 @@ __global__ void __launch_bounds__(512) route_batch_kernel(const __grid_constant_
     const uint32_t rows = min(a.per, a.tokens - row0);
     const uint32_t bad = route_rows<16>(row0, rows, E, k, a.norm, true, reinterpret_cast<float *>(rb_smem + sizeof(RouteShared)),
                    *reinterpret_cast<RouteShared *>(rb_smem), a.status, a.probs,
-                   [&](uint32_t t, uint32_t e) { return __ldg(a.logits + (uint64_t)t * a.pitch + e); },
+                   // past L1: the launch ahead may have read these lines on this SM before it wrote them (adapters on the logits)
+                   [&](uint32_t t, uint32_t e) { return __ldcg(a.logits + (uint64_t)t * a.pitch + e); },
                    [&](uint32_t t, uint32_t slot, uint32_t id, float w) {
                        const uint64_t at = (uint64_t)t * k + slot;
                        a.ids[at] = id; a.weights[at] = w;

@@ -55,3 +55,14 @@ def test_collectives_stay_where_they_are_written(source):
     which all lanes of a warp have to take part then never ends."""
     for m in re.finditer(r"\basm\s*\(\s*\"[^\"]*\b(redux|elect|vote|shfl|match|bar|barrier|activemask)\.", without_comments(source.read_text())):
         pytest.fail(f"{source.name}: collective in an asm that is not volatile: {m.group(0)}")
+
+
+@pytest.mark.parametrize("source", SOURCES, ids=lambda p: p.name)
+def test_kernels_launched_early_read_nothing_as_constant(source):
+    """A kernel that may begin before the launch ahead of it has ended runs while its inputs are written.  A load that is told otherwise (__ldg, or a
+    pointer to const that is __restrict__) may come before the wait, and may find a line that the SM kept from the launch ahead."""
+    weights = r"\(m \? a\.row_scale1 : a\.row_scale0\)"     # scales of the weights' rows, written when the layer was made
+    for head, body in functions(without_comments(source.read_text()), r"__global__"):
+        if "griddepcontrol.wait" in body or "grid_wait()" in body:
+            assert not re.search(r"\bconst\s[^,()]*__restrict__", head), head
+            assert not re.search(rf"__ldg\((?!{weights})", body), head
