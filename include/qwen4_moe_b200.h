@@ -545,7 +545,9 @@ size_t qw4cu_verify_pending(const QW4CuVerify *verify);
  * qw4cu_tune_work_reset.  Calls on one workspace must follow one another on the GPU (one stream, or
  * streams that wait for each other; graphs captured with it likewise); calls that may overlap need a
  * workspace each.  A workspace belongs to the device that was current when it was made.  Results
- * do not depend on timing: every sum has a fixed order.
+ * do not depend on timing: every sum has a fixed order.  An output must not share elements with what is read or with
+ * another output, unless said; columns of one wider buffer (rows of one pitch) share none, views of different pitches
+ * count as sharing some where their address ranges meet.
  * ---------------------------------------------------------------------------------- */
 typedef struct QW4CuTuneWork QW4CuTuneWork;
 

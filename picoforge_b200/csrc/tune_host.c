@@ -135,9 +135,9 @@ Qwen4Status qw4cu_tune_work_reset(QW4CuTuneWork *w, Qwen4Error *err) {
 }
 
 /* ---- arguments ---------------------------------------------------------------------------- */
-typedef struct { uintptr_t first, end; } Bytes;
+typedef struct { uintptr_t first, end; size_t rows, row, pitch; } Bytes;
 
-/* rows x row_bytes bytes, `pitch` bytes apart, as an address range; what is wrong with it, or NULL. */
+/* rows x row_bytes bytes, `pitch` bytes apart; what is wrong with it, or NULL. */
 static const char *view(const void *p, size_t rows, size_t row_bytes, size_t pitch, size_t align, Bytes *out, Qwen4Status *code) {
     *code = QW4_INVALID_ARGUMENT;
     if (!p) return "null device view";
@@ -148,10 +148,19 @@ static const char *view(const void *p, size_t rows, size_t row_bytes, size_t pit
     if (rows && pitch > (SIZE_MAX / 2 - row_bytes) / rows) return "extent overflow";
     const size_t bytes = rows ? (rows - 1) * pitch + row_bytes : 0;
     if ((uintptr_t)p + bytes < (uintptr_t)p) return "address overflow";
-    *out = (Bytes){(uintptr_t)p, (uintptr_t)p + bytes};
+    *out = (Bytes){(uintptr_t)p, (uintptr_t)p + bytes, rows, row_bytes, pitch};
     return NULL;
 }
-static bool meet(Bytes a, Bytes b) { return a.first < b.end && b.first < a.end; }
+/* Whether two views share a byte.  Rows of one pitch can lie between one another (columns of a wider buffer); of different pitches they are
+ * taken to meet where the address ranges do. */
+static bool meet(Bytes a, Bytes b) {
+    if (a.first >= b.end || b.first >= a.end) return false;
+    if (a.first > b.first) { const Bytes c = a; a = b; b = c; }
+    if (a.rows == 1) return true;                                    /* b begins inside the only row */
+    if (b.rows > 1 && a.pitch != b.pitch) return true;
+    const size_t into = (b.first - a.first) % a.pitch;               /* b begins in a row of a, or behind one and reaches the next */
+    return into < a.row || into + b.row > a.pitch;
+}
 #define VIEW(p, rows, row_bytes, pitch, align, out) do { Qwen4Status code_; const char *bad_ = view((p), (rows), (row_bytes), (pitch), (align), (out), &code_); \
     if (bad_) return answer(err, code_, bad_); } while (0)
 #define TRY(call) do { const Qwen4Status st_ = (call); if (st_ != QW4_OK) return st_; } while (0)
@@ -162,7 +171,7 @@ static Qwen4Status usable(const QW4CuTuneWork *w, size_t tokens, void **stream, 
     if (tokens > w->limits.tokens) return answer(err, QW4_CAPACITY, "batch exceeds the workspace's tokens");
     return stream_of(w, stream, err);
 }
-/* Every written range apart from every other range, except that written[same_w] may be read[same_r] (the same rows). */
+/* Every written view apart from every other view, except that written[same_w] may be read[same_r] (the same rows). */
 static Qwen4Status apart(const Bytes *written, size_t nw, const Bytes *read, size_t nr, size_t same_w, size_t same_r, Qwen4Error *err) {
     for (size_t i = 0; i < nw; i++) {
         for (size_t j = 0; j < nr; j++)
@@ -182,7 +191,7 @@ static Qwen4Status check_adapters(const QW4CuAdapters *ad, const QW4CuTuneWork *
     const size_t e = ad->type == 0 ? 4 : 2;
     VIEW(ad->a, ad->slots, ad->rank * ad->k * e, ad->rank * ad->k * e, e, a);
     VIEW(ad->b, ad->slots, ad->rank * ad->n * e, ad->rank * ad->n * e, e, b);
-    *scale = (Bytes){0, 0};
+    *scale = (Bytes){0};
     if (ad->scale) VIEW(ad->scale, 1, ad->slots * 4, ad->slots * 4, 4, scale);
     return QW4_OK;
 }
@@ -203,7 +212,7 @@ Qwen4Status qw4cu_adapter_forward_device(const QW4CuAdapters *ad, const float *x
                                          size_t base_pitch, float *y, size_t y_pitch, size_t tokens, QW4CuTuneWork *w, Qwen4Error *err) {
     void *stream;
     TRY(usable(w, tokens, &stream, err));
-    Bytes read[6] = {{0, 0}}, out;
+    Bytes read[6] = {{0}}, out;
     TRY(check_adapters(ad, w, &read[0], &read[1], &read[2], err));
     if (!tokens) return answer(err, QW4_OK, "");
     VIEW(x, tokens, ad->k * 4, x_pitch, 4, &read[3]);
@@ -220,7 +229,7 @@ Qwen4Status qw4cu_adapter_backward_device(const QW4CuAdapters *ad, const float *
                                           size_t tokens, QW4CuTuneWork *w, Qwen4Error *err) {
     void *stream;
     TRY(usable(w, tokens, &stream, err));
-    Bytes read[7] = {{0, 0}}, out[3] = {{0, 0}};
+    Bytes read[7] = {{0}}, out[3] = {{0}};
     TRY(check_adapters(ad, w, &read[0], &read[1], &read[2], err));
     if (!da != !db) return answer(err, QW4_INVALID_ARGUMENT, "da and db are given together");
     if (!dx && !da) return answer(err, QW4_INVALID_ARGUMENT, "no gradient asked for");
@@ -253,7 +262,7 @@ Qwen4Status qw4cu_balance_forward_device(const Qwen4MoeConfig *c, const float *l
     void *stream;
     TRY(usable(w, tokens, &stream, err));
     TRY(check_router(c, w, err));
-    Bytes read[3] = {{0, 0}}, out[3];
+    Bytes read[3] = {{0}}, out[3];
     const size_t e = c->experts;
     if (tokens) {
         VIEW(logits, tokens, e * 4, pitch, 4, &read[0]);
@@ -276,7 +285,7 @@ Qwen4Status qw4cu_balance_backward_device(const Qwen4MoeConfig *c, const float *
     TRY(usable(w, tokens, &stream, err));
     TRY(check_router(c, w, err));
     if (!tokens) return answer(err, QW4_OK, "");
-    Bytes read[5] = {{0, 0}}, out;
+    Bytes read[5] = {{0}}, out;
     const size_t e = c->experts, pairs = tokens * c->top_k;
     VIEW(logits, tokens, e * 4, pitch, 4, &read[0]);
     VIEW(ids, 1, pairs * 4, pairs * 4, 4, &read[1]);
