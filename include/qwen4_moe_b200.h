@@ -600,7 +600,7 @@ Qwen4Status qw4cu_adapter_backward_device(const QW4CuAdapters *adapters, const f
 /* The layer's own router with the requests' adapters (k = hidden size, n = experts) beside it: logits of the router, scale B (A x) of every
  * token's slot on top, then the routes and, in the second call, the whole layer on them.  adapters NULL: the plain router (slots_dev and tune are
  * then not looked at).  logits_dev [tokens, experts], ids_dev and weights_dev [tokens, top_k] may be NULL; logits_dev receives what was
- * routed, which is what the balance loss wants.  Otherwise as qw4cu_moe_route_device and qw4cu_moe_forward_device, for up to 2048 tokens, without
+ * routed, which is what the balance loss wants, and must lie apart from every other argument.  Otherwise as qw4cu_moe_route_device and qw4cu_moe_forward_device, for up to 2048 tokens, without
  * the one-kernel decode path and without replay; bad slots are reported by qw4cu_tune_work_sync, everything else by qw4cu_moe_work_sync. */
 Qwen4Status qw4cu_moe_route_adapted_device(const Qwen4Moe *moe, const float *x_dev, size_t tokens, const QW4CuAdapters *adapters,
                                            const uint32_t *slots_dev, QW4CuTuneWork *tune, float *logits_dev, uint32_t *ids_dev,

@@ -265,6 +265,9 @@ size_t qw4sh_adapter_rows(size_t tokens, uint32_t slots);
  * qw4cu_adapter_forward_device on what is given here. */
 Qwen4Status qw4tune_beside(const QW4CuAdapters *adapters, size_t k, size_t n, const uint32_t *slots, size_t tokens, QW4CuTuneWork *work,
                            const QW4ShTune **tune, Qwen4Error *err);
+/* tune_host.c: whether `logits` (or NULL) may receive [tokens, experts] beside the other arguments of a layer call with adapters. */
+Qwen4Status qw4tune_logits_out(const float *logits, size_t tokens, size_t hidden, size_t experts, size_t top_k, const float *x, const float *y,
+                               const uint32_t *ids, const float *weights, const QW4CuAdapters *adapters, const uint32_t *slots, Qwen4Error *err);
 size_t qw4sh_adapter_tiles(size_t tokens, uint32_t slots);
 uint32_t qw4sh_adapter_rank(uint32_t rank);
 int qw4sh_balance_forward(const QW4ShTune *tune, uint32_t experts, uint32_t k, const float *logits, size_t pitch, const uint32_t *ids,

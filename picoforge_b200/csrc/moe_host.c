@@ -526,6 +526,7 @@ static Qwen4Status adapted(const Qwen4Moe *m, const float *x_dev, float *y_dev, 
     TRY(piece_checks(m, w, tokens, err));
     const QW4ShTune *scratch = NULL;
     if (adapters) TRY(qw4tune_beside(adapters, m->c.hidden_size, m->c.experts, slots_dev, tokens, tune, &scratch, err));
+    if (tokens) TRY(qw4tune_logits_out(logits_dev, tokens, m->c.hidden_size, m->c.experts, m->c.top_k, x_dev, y_dev, ids_dev, weights_dev, adapters, slots_dev, err));
     w->d.router_adapters = tokens ? adapters : NULL; w->d.router_slots = slots_dev; w->d.router_tune = scratch; w->d.logits_out = tokens ? logits_dev : NULL;
     const Qwen4Status st = route_only ? qw4cu_moe_route_device(m, x_dev, tokens, ids_dev, weights_dev, w, err)
                                       : qw4cu_moe_forward_device(m, x_dev, y_dev, tokens, ids_dev, weights_dev, w, err);

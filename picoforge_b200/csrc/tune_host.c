@@ -208,6 +208,22 @@ Qwen4Status qw4tune_beside(const QW4CuAdapters *ad, size_t k, size_t n, const ui
     return QW4_OK;
 }
 
+static Bytes dense(const void *p, size_t bytes) { return p ? (Bytes){(uintptr_t)p, (uintptr_t)p + bytes, 1, bytes, bytes} : (Bytes){0}; }
+Qwen4Status qw4tune_logits_out(const float *logits, size_t tokens, size_t hidden, size_t experts, size_t top_k, const float *x, const float *y,
+                               const uint32_t *ids, const float *weights, const QW4CuAdapters *ad, const uint32_t *slots, Qwen4Error *err) {
+    if (!logits) return answer(err, QW4_OK, "");
+    Bytes out, others[8] = {dense(x, tokens * hidden * 4), dense(y, tokens * hidden * 4), dense(ids, tokens * top_k * 4), dense(weights, tokens * top_k * 4)};
+    if (ad) {
+        const size_t e = ad->type == 0 ? 4 : 2;
+        others[4] = dense(slots, tokens * 4);
+        others[5] = dense(ad->a, ad->slots * ad->rank * ad->k * e);
+        others[6] = dense(ad->b, ad->slots * ad->rank * ad->n * e);
+        others[7] = dense(ad->scale, ad->slots * 4);
+    }
+    VIEW(logits, 1, tokens * experts * 4, tokens * experts * 4, 4, &out);
+    return apart(&out, 1, others, 8, 1, 8, err) == QW4_OK ? answer(err, QW4_OK, "") : answer(err, QW4_INVALID_ARGUMENT, "the logits overlap another argument");
+}
+
 Qwen4Status qw4cu_adapter_forward_device(const QW4CuAdapters *ad, const float *x, size_t x_pitch, const uint32_t *slots, const float *base,
                                          size_t base_pitch, float *y, size_t y_pitch, size_t tokens, QW4CuTuneWork *w, Qwen4Error *err) {
     void *stream;

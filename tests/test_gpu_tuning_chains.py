@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from cases import small_layer
-from picoforge_b200 import tuning
+from picoforge_b200 import abi, tuning
 from test_gpu_adapted_layer import Setup, api  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +59,28 @@ def test_balance_loss_behind_adapters_in_place(api, experts, tokens):  # noqa: F
         for _ in range(4):
             for p, q in zip(want, chain(False)):
                 assert torch.equal(p, q)
+
+
+def test_logits_handed_out_over_another_argument(api):  # noqa: F811
+    """Refused before anything is launched, and the calls after it are as ever."""
+    s = Setup(api, small_layer(22), 20)
+    s.forward()
+    s.sync(api)
+    want = s.y.clone(), s.ids.clone(), s.logits.clone()
+    api.lib.qw4cu_launch_log_begin()
+    def forward(logits):
+        s.tune.layer_forward(s.layer, s.view, s.x.data_ptr(), s.slot.data_ptr(), s.y.data_ptr(), s.t, logits.data_ptr(), s.ids.data_ptr(), s.weights.data_ptr())
+
+    def route(logits):
+        s.tune.route(s.layer, s.view, s.x.data_ptr(), s.slot.data_ptr(), s.t, logits.data_ptr(), s.ids.data_ptr(), s.weights.data_ptr())
+    for call, others in ((forward, (s.x, s.y, s.ids, s.weights, s.slot, s.a, s.b)), (route, (s.x, s.ids, s.weights, s.slot, s.a, s.b))):
+        for logits in others:
+            with pytest.raises(abi.MoeError) as info:
+                call(logits)
+            assert info.value.status == abi.INVALID_ARGUMENT
+    assert not api.launch_names()
+    s.forward()
+    s.sync(api)
+    for p, q in zip(want, (s.y, s.ids, s.logits)):
+        assert torch.equal(p, q)
+    s.close()
