@@ -18,7 +18,16 @@ extern "C" int qw4sh_allow_smem(const void *kernel, size_t smem);
 namespace {
 
 constexpr uint32_t THREADS = 256;
-constexpr float UNIT = 1099511627776.0f;          // 2^40: probability sums meet as 64-bit integers, whose sum has no order
+
+// Probability sums meet as 64-bit integers, whose sum has no order: multiples of 2^-40 in the first, and what is left of a share in multiples of
+// 2^-82 in the second, so that an unlikely expert's sum keeps FP32's bits too.  A share of 2^-16 and more has nothing left.  Neither
+// overflows: shares add up to no more than 2^20 tokens, and there are no more than that many of less than 2^42 each in the second.
+constexpr float UNIT = 1099511627776.0f, REST = 4835703278458516698824704.0f;        // 2^40, 2^82
+__device__ __forceinline__ void add_share(unsigned long long *sum, uint32_t to_rest, float v) {
+    const long long whole = __float2ll_rz(v * UNIT), rest = __float2ll_rn(fmaf((float)whole, -1.0f / UNIT, v) * REST);        // both exact but for the last rounding
+    if (whole) atomicAdd(sum, (unsigned long long)whole);
+    if (rest) atomicAdd(sum + to_rest, (unsigned long long)rest);
+}
 
 // By all lanes of a warp together: volatile, or the compiler may move it to where its result is used, which not every lane reaches.
 __device__ __forceinline__ float warp_max(float v) {
@@ -95,11 +104,11 @@ __device__ __forceinline__ void balance_finish(uint32_t E, const QW4ShTune &tune
     double l = 0;
     for (uint32_t e = threadIdx.x; e < E; e += THREADS) {
         const uint32_t c = __ldcg(&tune.counts[e]);
-        const double p = (double)__ldcg(&tune.prob_sums[e]) * (1.0 / (double)UNIT);
+        const double p = (double)__ldcg(&tune.prob_sums[e]) * (1.0 / (double)UNIT) + (double)__ldcg(&tune.prob_sums[E + e]) * (1.0 / (double)REST);
         counts[e] = c;
         prob_sums[e] = bad ? CUDART_NAN_F : (float)p;
         l += (double)c * p;
-        tune.counts[e] = 0; tune.prob_sums[e] = 0;
+        tune.counts[e] = 0; tune.prob_sums[e] = tune.prob_sums[E + e] = 0;
     }
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     if (lane == 0) part[warp] = l;
@@ -166,8 +175,7 @@ __global__ void __launch_bounds__(THREADS) balance_forward_kernel(uint32_t E, ui
         float sum = 0;
 #pragma unroll
         for (uint32_t w = 0; w < WARPS; w++) sum += sums[w * COLS + e];
-        const unsigned long long u = (unsigned long long)__float2ll_rn(sum * UNIT);
-        if (u) atomicAdd(&tune.prob_sums[e], u);
+        add_share(&tune.prob_sums[e], E, sum);
         if (hist[e]) atomicAdd(&tune.counts[e], hist[e]);
     }
     if (threadIdx.x == 0 && rows_seen) atomicAdd(&tune.counts[E], rows_seen);
@@ -180,12 +188,12 @@ __global__ void __launch_bounds__(THREADS) balance_forward_wide_kernel(uint32_t 
                                                                        const uint32_t *ids, const uint8_t *mask, uint32_t T,
                                                                        const __grid_constant__ QW4ShTune tune, uint32_t *__restrict__ counts,
                                                                        float *__restrict__ prob_sums, float *__restrict__ loss) {
-    extern __shared__ uint32_t shared_words[];               // [E] counts, [E] sums as 64-bit integers
+    extern __shared__ uint32_t shared_words[];               // [E] counts, [2][E] sums as 64-bit integers
     uint32_t *hist = shared_words;
     unsigned long long *sums = (unsigned long long *)(hist + ((E + 1) & ~1u));
     __shared__ uint32_t rows_seen;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (uint32_t e = threadIdx.x; e < E; e += THREADS) { hist[e] = 0; sums[e] = 0; }
+    for (uint32_t e = threadIdx.x; e < E; e += THREADS) { hist[e] = 0; sums[e] = sums[E + e] = 0; }
     if (threadIdx.x == 0) rows_seen = 0;
     grid_wait();
     __syncthreads();
@@ -199,7 +207,7 @@ __global__ void __launch_bounds__(THREADS) balance_forward_wide_kernel(uint32_t 
         s = warp_sum(s);
         if (!(s < CUDART_INF_F)) { if (lane == 0) { note_nonfinite(tune.status, t); tune.status[2] = 1; } }
         const float inv = 1.0f / s;
-        for (uint32_t e = lane; e < E; e += 32) atomicAdd(&sums[e], (unsigned long long)__float2ll_rn(expf(z[e] - m) * inv * UNIT));
+        for (uint32_t e = lane; e < E; e += 32) add_share(&sums[e], E, expf(z[e] - m) * inv);
         for (uint32_t k = lane; k < K; k += 32) {
             const uint32_t e = ids[(uint64_t)t * K + k];
             if (e < E) atomicAdd(&hist[e], 1u); else atomicOr(tune.status, QW4SH_ERR_BOUNDS);
@@ -210,6 +218,7 @@ __global__ void __launch_bounds__(THREADS) balance_forward_wide_kernel(uint32_t 
     for (uint32_t e = threadIdx.x; e < E; e += THREADS) {
         if (hist[e]) atomicAdd(&tune.counts[e], hist[e]);
         if (sums[e]) atomicAdd(&tune.prob_sums[e], sums[e]);
+        if (sums[E + e]) atomicAdd(&tune.prob_sums[E + e], sums[E + e]);
     }
     if (threadIdx.x == 0 && rows_seen) atomicAdd(&tune.counts[E], rows_seen);
     balance_finish(E, tune, counts, prob_sums, loss);
@@ -394,7 +403,7 @@ extern "C" int qw4sh_balance_forward(const QW4ShTune *tune, uint32_t E, uint32_t
                                 (uint32_t)tokens, *tune, counts, prob_sums, loss)
     if (E <= 1024) return BY_ROW(balance_forward_kernel, RUN);
 #undef RUN
-    return launch(balance_forward_wide_kernel, "balance_forward_wide_kernel", grid_of(tokens, 4), (size_t)((E + 1) & ~1u) * 4 + (size_t)E * 8, stream, E, K, logits,
+    return launch(balance_forward_wide_kernel, "balance_forward_wide_kernel", grid_of(tokens, 4), (size_t)((E + 1) & ~1u) * 4 + (size_t)E * 16, stream, E, K, logits,
                   pitch, ids, mask, (uint32_t)tokens, *tune, counts, prob_sums, loss);
 }
 

@@ -251,7 +251,7 @@ int qw4sh_route_forward(const QW4ShLayer *layer, const QW4ShWork *work, const fl
 struct QW4ShTune {
     uint32_t *status;             /* [4]: error bits, lowest bad row, whether this forward pass of the loss met one */
     /* balance loss: sums over the CTAs of a launch, zero between launches */
-    unsigned long long *prob_sums;    /* [experts] units of 2^-40 */
+    unsigned long long *prob_sums;    /* [2][experts of the call]: units of 2^-40, then of 2^-82 */
     uint32_t *counts;             /* [experts + 1], and one ticket behind them */
     /* adapters: tokens sorted by slot, and tiles of them (16 bytes each) */
     uint32_t *order, *offsets;    /* [qw4sh_adapter_rows(tokens, slots)], [slots + 1][start, tokens] */
