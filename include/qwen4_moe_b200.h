@@ -585,7 +585,9 @@ typedef struct {
 /* y[t] = base[t] + scale_s B_s (A_s x[t]) with s = slots_dev[t]; y[t] = base[t] where that is QW4CU_NO_ADAPTER (or
  * out of range).  base NULL: zero; base may be y itself (same pitch), otherwise y must not overlap what is read.
  * Pitches are bytes between rows.  x [tokens, k], base and y [tokens, n].  Tokens of a slot may lie anywhere in the
- * batch.  Values enter the products with all their bits and are summed in FP32 (of products of two FP32 values 2^-21 at most is left out). */
+ * batch.  Values enter the products with all their bits and are summed in FP32 (of products of two FP32 values 2^-21 at most is left out).
+ * An infinity or a NaN in an operand, and a sum beyond FP32's range, make those results not finite that the formula takes them to, and no others;
+ * which of an infinity and a NaN comes out is not said and may depend on the number of tokens.  The same holds for the gradients. */
 Qwen4Status qw4cu_adapter_forward_device(const QW4CuAdapters *adapters, const float *x_dev, size_t x_pitch, const uint32_t *slots_dev,
                                          const float *base_dev, size_t base_pitch, float *y_dev, size_t y_pitch, size_t tokens,
                                          QW4CuTuneWork *work, Qwen4Error *err);
