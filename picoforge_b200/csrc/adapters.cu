@@ -30,7 +30,7 @@ extern "C" int qw4sh_allow_smem(const void *kernel, size_t smem);
 namespace {
 
 constexpr uint32_t THREADS = 256, TM = 128;                  // tokens per tile: tcgen05's M (shrink) or most N (expand)
-constexpr uint32_t KC = 64, AHEAD = 1;                       // shrink: columns per step, steps that x is fetched ahead
+constexpr uint32_t KC = 64;                                  // shrink: columns per step
 constexpr uint32_t TC = 64;                                  // outer: tokens per step
 
 // ---- PTX ------------------------------------------------------------------------------------------------------------------
@@ -202,8 +202,7 @@ template <uint32_t BYTES> __device__ __forceinline__ void copy_async(uint32_t ds
     if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(there), "n"(BYTES) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // How many of four places from c on lie before `end`.
 __device__ __forceinline__ int places(uint32_t c, uint32_t end) { return c < end ? (int)min(4u, end - c) : 0; }
@@ -213,7 +212,7 @@ __device__ __forceinline__ int places(uint32_t c, uint32_t end) { return c < end
 template <typename W> struct Mat { const W *p; uint64_t slot; uint32_t rank, width; bool wide, fours; };
 
 // A run of LEN columns of a slot's matrix (rank padded to RP) on its way into the operand tiles Wide (RP x LEN) or Tall (LEN x RP).
-// Where runs of four lie on their boundaries a thread keeps the places it reads in such runs and moves them on from run to run.
+// Where runs of four lie on their boundaries a thread keeps the places it reads in such runs (and `copy` moves them on from run to run).
 template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
     static constexpr uint32_t ALL = RP * LEN / 4, UNITS = (ALL + THREADS - 1) / THREADS, PLANES = Four<W>::PLANES;
     using Wide = Tile<RP, LEN, PLANES>;
@@ -221,7 +220,7 @@ template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
     static constexpr uint32_t BYTES = Wide::BYTES > Tall::BYTES ? Wide::BYTES : Tall::BYTES;
     Four<W> v[UNITS];
     uint32_t at[UNITS];
-    static __device__ __forceinline__ bool idle() { return ALL < THREADS && threadIdx.x >= ALL; }           // fewer runs of four than threads
+    static_assert(ALL >= THREADS, "no thread without a run of four");
     static __device__ __forceinline__ uint32_t wide_r(uint32_t i) { return (threadIdx.x + i * THREADS) / (LEN / 4); }
     static __device__ __forceinline__ uint32_t wide_c(uint32_t i) { return (threadIdx.x + i * THREADS) % (LEN / 4) * 4; }
     static __device__ __forceinline__ uint32_t tall_c(uint32_t i) { return (threadIdx.x + i * THREADS) / (RP / 4); }
@@ -231,13 +230,11 @@ template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
         for (uint32_t i = 0; i < UNITS; i++)
             at[i] = m.wide ? (min(wide_r(i), m.rank - 1) * m.width + c0 + wide_c(i)) / 4 : ((c0 + tall_c(i)) * m.rank + min(tall_r(i), (m.rank - 1) & ~3u)) / 4;
     }
-    // columns c0 .. c0 + LEN of w, which end at `end`
+    // columns c0 .. c0 + LEN of w, which end at `end`; where m.fours, the ones that `begin` was told
     __device__ __forceinline__ void load(const Mat<W> &m, const W *w, uint32_t c0, uint32_t end) {
-        if (idle()) return;
         if (m.fours && c0 + LEN <= end) {
-            const uint32_t step = m.wide ? LEN / 4 : LEN / 4 * m.rank;
 #pragma unroll
-            for (uint32_t i = 0; i < UNITS; i++) { v[i].load4(w + (uint64_t)at[i] * 4); at[i] += step; }
+            for (uint32_t i = 0; i < UNITS; i++) v[i].load4(w + (uint64_t)at[i] * 4);
         } else if (m.wide) {
 #pragma unroll 1
             for (uint32_t i = 0; i < UNITS; i++) {
@@ -256,7 +253,6 @@ template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
     }
     // the same by way of the thread's own places in shared memory, UNITS of them `stride` bytes apart; only where m.fours
     __device__ __forceinline__ void copy(const Mat<W> &m, const W *w, uint32_t c0, uint32_t end, uint32_t to, uint32_t stride) {
-        if (idle()) return;
         const uint32_t step = m.wide ? LEN / 4 : LEN / 4 * m.rank;
 #pragma unroll
         for (uint32_t i = 0; i < UNITS; i++) {
@@ -274,7 +270,6 @@ template <typename W, uint32_t RP, uint32_t LEN> struct MatRun {
         for (uint32_t j = 0; j < UNITS; j++) if (i == j) v[j] = f;
     }
     __device__ __forceinline__ void put(const Mat<W> &m, uint32_t c0, uint32_t end, uint32_t addr) {
-        if (idle()) return;
         if (m.rank != RP || c0 + LEN > end)
 #pragma unroll
             for (uint32_t i = 0; i < UNITS; i++) {
@@ -485,12 +480,12 @@ template <typename W, uint32_t RP> struct ShrinkMap {
     static constexpr uint32_t XU = TM * KC / 4 / THREADS;    // runs of four values of x per thread and step
     static constexpr uint32_t W_UNIT = THREADS * 4 * sizeof(W), SLOT = XU * THREADS * 16 + Run::UNITS * W_UNIT;
     static constexpr uint32_t OPERANDS = X::BYTES + Run::BYTES;
-    static constexpr uint32_t ORDER = 64, STAGE = ORDER + TM * 4, RING = STAGE + OPERANDS, END = RING + AHEAD * SLOT;
+    static constexpr uint32_t ORDER = 64, STAGE = ORDER + TM * 4, RING = STAGE + OPERANDS, END = RING + SLOT;
     static constexpr uint32_t PITCH = RP + 4;                // floats per row of the exchanged accumulators
     static constexpr uint32_t ACC_END = STAGE + TM * PITCH * 4, TOTAL = END > ACC_END ? END : ACC_END;
 };
 
-// Values come in by asynchronous copies, AHEAD steps before they are cut, each thread's own into places of its own: no barrier, no register and no line
+// Values come in by asynchronous copies, a step before they are cut, each thread's own into places of its own: no barrier, no register and no line
 // of L1 holds them meanwhile (through registers an SM had half as many bytes under way).
 template <typename W, uint32_t RP>
 __global__ void __launch_bounds__(THREADS, RP <= 64 ? 2 : 1) adapter_shrink_kernel(const __grid_constant__ ShrinkArgs<W> a) {
@@ -528,13 +523,13 @@ __global__ void __launch_bounds__(THREADS, RP <= 64 ? 2 : 1) adapter_shrink_kern
     const float *x = job.x;
     auto copy = [&](uint32_t s) {
         if (s < steps) {
-            const uint32_t c = c_first + s * KC + x_col, slot = s % AHEAD * M::SLOT;
+            const uint32_t c = c_first + s * KC + x_col;
             const uint32_t valid = places(c, c_end);
             if (job.x_fours) {
 #pragma unroll
                 for (uint32_t i = 0; i < XU; i++) {
                     const bool there = x_row + i * ROWS < t.rows && valid;
-                    copy_async<16>(mine + slot + i * THREADS * 16, there ? x + (uint64_t)x_at[i] * 4 : x, there ? 4 * valid : 0);
+                    copy_async<16>(mine + i * THREADS * 16, there ? x + (uint64_t)x_at[i] * 4 : x, there ? 4 * valid : 0);
                     x_at[i] += KC / 4;
                 }
             } else {
@@ -544,31 +539,29 @@ __global__ void __launch_bounds__(THREADS, RP <= 64 ? 2 : 1) adapter_shrink_kern
 #pragma unroll
                     for (uint32_t j = 0; j < 4; j++) {
                         const bool there = x_row + i * ROWS < t.rows && j < valid;
-                        copy_async<4>(mine + slot + i * THREADS * 16 + 4 * j, there ? row + c + j : x, there ? 4 : 0);
+                        copy_async<4>(mine + i * THREADS * 16 + 4 * j, there ? row + c + j : x, there ? 4 : 0);
                     }
                 }
             }
-            if (m.fours) wv.copy(m, w, c_first + s * KC, c_end, mine_w + slot, M::W_UNIT);
+            if (m.fours) wv.copy(m, w, c_first + s * KC, c_end, mine_w, M::W_UNIT);
         }
-        copies_commit();
     };
-#pragma unroll
-    for (uint32_t s = 0; s < AHEAD; s++) copy(s);
+    copy(0);
     const uint32_t idesc = idesc_of(TM, RP, false, !m.wide);
     for (uint32_t s = 0; s < steps; s++) {
-        const uint32_t c0 = c_first + s * KC, slot = s % AHEAD * M::SLOT, at = base + M::STAGE, wat = at + M::X::BYTES;
-        copies_wait<AHEAD - 1>();
+        const uint32_t c0 = c_first + s * KC, at = base + M::STAGE, wat = at + M::X::BYTES;
+        copies_wait();
         if (s) bar_wait(base, (s - 1) & 1, a.status);
         if (s && s % FLUSH == 0) flush<RP>(tmem, s > FLUSH);
 #pragma unroll
         for (uint32_t i = 0; i < XU; i++) {
             Four<float> xv;
-            xv.take(mine + slot + i * THREADS * 16);
+            xv.take(mine + i * THREADS * 16);
             xv.put(at + M::X::at(x_row + i * ROWS, x_col), M::X::PLANE);
         }
-        if (m.fours) wv.take(mine_w + slot, M::W_UNIT); else wv.load(m, w, c0, c_end);
+        if (m.fours) wv.take(mine_w, M::W_UNIT); else wv.load(m, w, c0, c_end);
         wv.put(m, c0, c_end, wat);
-        copy(s + AHEAD);
+        copy(s + 1);
         fence_async();
         __syncthreads();
         if (warp == 0) {
@@ -580,7 +573,7 @@ __global__ void __launch_bounds__(THREADS, RP <= 64 ? 2 : 1) adapter_shrink_kern
             __syncwarp();
         }
     }
-    copies_wait<0>();
+    copies_wait();
     if (steps) bar_wait(base, (steps - 1) & 1, a.status);
     tc_after();
     grid_go();                                               // not before: CTAs of the next launch would crowd onto the SMs that are done first
@@ -630,7 +623,7 @@ template <typename W> struct ExpandArgs {
     const __nv_bfloat16 *planes;                             // of shrink
     uint64_t plane;
     Lists lists;
-    uint32_t slots, blocks;                                  // blocks of 128 columns per CTA
+    uint32_t slots;
     const float *base;
     uint64_t base_pitch;
     float *y;
@@ -663,7 +656,7 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
     const bool none = t.slot >= a.slots;
     if (none && a.base == a.y) { grid_wait(); return; }
     const Mat<W> m = a.w;
-    const uint32_t first = blockIdx.x * a.blocks, last = min((m.width + 127) / 128, first + a.blocks);
+    const uint32_t c0 = blockIdx.x * 128, c = c0 + (warp & 3) * 32 + lane;
     if (tid < 2) bar_init(base + 8 * tid);                   // products, rows of shrink
     if (tid < TM) {
         const uint64_t row = a.lists.order[t.first + min(tid, t.rows - 1)];
@@ -673,8 +666,8 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
     typename M::Run wv;
     const uint32_t n = uniform((t.rows + 15) & ~15u);
     if (!none) {
-        wv.begin(m, first * 128);
-        wv.load(m, w, first * 128, m.width);
+        wv.begin(m, c0);
+        wv.load(m, w, c0, m.width);
     }
     if (warp == 0) tc_alloc(base + 32, TM);
     tc_before();
@@ -688,49 +681,44 @@ __global__ void __launch_bounds__(THREADS, ExpandMap<W, RP>::CTAS) adapter_expan
     const uint32_t idesc = idesc_of(128, n, m.wide, false);
     const uint32_t t_first = (warp >> 2) * 64, t_last = min(t.rows, t_first + 64), d = tmem + ((warp & 3) << 21);
     const bool added = a.base != nullptr;
-    for (uint32_t block = first; block < last; block++) {
-        const uint32_t c = block * 128 + (warp & 3) * 32 + lane;
-        const char *b_col = (const char *)(a.base + min(c, m.width - 1));
-        char *y_col = (char *)(a.y + c);
-        float b[16], v[16];
-        auto fetch = [&](uint32_t j) {
+    const char *b_col = (const char *)(a.base + min(c, m.width - 1));
+    char *y_col = (char *)(a.y + c);
+    float b[16], v[16];
+    auto fetch = [&](uint32_t j) {
 #pragma unroll
-            for (uint32_t i = 0; i < 16; i++) b[i] = *(const float *)(b_col + place[j + i].b);
-        };
-        if (added && t_first < t_last && (none || block == first)) fetch(t_first);
-        if (!none) {
-            wv.put(m, block * 128, m.width, base + M::W_AT);
-            fence_async();
-            tc_before();
-            __syncthreads();
-            if (warp == 0) {
-                tc_after();
-                if (block == first) bar_wait(base + 8, 0, a.status);
-                __syncwarp();
-                const uint32_t leader = elect();
-                if (m.wide) step_mma<typename M::Run::Wide, typename M::H, M::Run::PLANES, 3, true, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
-                else step_mma<typename M::Run::Tall, typename M::H, M::Run::PLANES, 3, false, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
-                if (leader) tc_commit(base);
-                __syncwarp();
-            }
-            if (added && t_first < t_last && block != first) fetch(t_first);
-            if (block + 1 < last) wv.load(m, w, (block + 1) * 128, m.width);
-            bar_wait(base, (block - first) & 1, a.status);
+        for (uint32_t i = 0; i < 16; i++) b[i] = *(const float *)(b_col + place[j + i].b);
+    };
+    if (added && t_first < t_last) fetch(t_first);
+    if (!none) {
+        wv.put(m, c0, m.width, base + M::W_AT);
+        fence_async();
+        tc_before();
+        __syncthreads();
+        if (warp == 0) {
             tc_after();
+            bar_wait(base + 8, 0, a.status);
+            __syncwarp();
+            const uint32_t leader = elect();
+            if (m.wide) step_mma<typename M::Run::Wide, typename M::H, M::Run::PLANES, 3, true, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
+            else step_mma<typename M::Run::Tall, typename M::H, M::Run::PLANES, 3, false, false, 1, RP / 16>(tmem, 0, tmem, base + M::W_AT, base + M::H_AT, idesc, true, leader);
+            if (leader) tc_commit(base);
+            __syncwarp();
         }
-        for (uint32_t j = t_first; j < t_last; j += 16) {
-            if (none) {
+        bar_wait(base, 0, a.status);
+        tc_after();
+    }
+    for (uint32_t j = t_first; j < t_last; j += 16) {
+        if (none) {
 #pragma unroll
-                for (uint32_t i = 0; i < 16; i++) v[i] = 0;
-            } else tc_load16(d + j, v);
-            if (added)
+            for (uint32_t i = 0; i < 16; i++) v[i] = 0;
+        } else tc_load16(d + j, v);
+        if (added)
 #pragma unroll
-                for (uint32_t i = 0; i < 16; i++) v[i] = none ? b[i] : b[i] + v[i];
-            if (added && j + 16 < t_last) fetch(j + 16);
-            if (c < m.width)
+            for (uint32_t i = 0; i < 16; i++) v[i] = none ? b[i] : b[i] + v[i];
+        if (added && j + 16 < t_last) fetch(j + 16);
+        if (c < m.width)
 #pragma unroll
-                for (uint32_t i = 0; i < 16; i++) if (j + i < t_last) *(float *)(y_col + place[j + i].y) = v[i];
-        }
+            for (uint32_t i = 0; i < 16; i++) if (j + i < t_last) *(float *)(y_col + place[j + i].y) = v[i];
     }
     tc_before();
     __syncthreads();
@@ -1110,11 +1098,8 @@ int shrink(const ShrinkJob<W> *jobs, uint32_t all, uint32_t n, const Shape &s) {
 }
 template <typename W, uint32_t RP>
 int expand(const Mat<W> &w, const __nv_bfloat16 *planes, const float *base, size_t base_pitch, float *y, size_t y_pitch, const Shape &s) {
-    ExpandArgs<W> a = {w, planes, s.plane, s.lists, s.S, 1, base, base_pitch, y, y_pitch, s.status};
-    const uint64_t blocks = (w.width + 127) / 128;
-    a.blocks = 1;
-    return launch(adapter_expand_kernel<W, RP>, "adapter_expand_kernel", dim3((unsigned)((blocks + a.blocks - 1) / a.blocks), s.tiles), THREADS,
-                  ExpandMap<W, RP>::TOTAL, 0, true, s.stream, a);
+    const ExpandArgs<W> a = {w, planes, s.plane, s.lists, s.S, base, base_pitch, y, y_pitch, s.status};
+    return launch(adapter_expand_kernel<W, RP>, "adapter_expand_kernel", dim3((w.width + 127) / 128, s.tiles), THREADS, ExpandMap<W, RP>::TOTAL, 0, true, s.stream, a);
 }
 template <uint32_t RP>
 int outer(const OuterJob *jobs, const Shape &s) {
