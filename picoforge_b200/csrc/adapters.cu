@@ -487,6 +487,7 @@ template <typename W, uint32_t RP> struct ShrinkMap {
 
 // Values come in by asynchronous copies, a step before they are cut, each thread's own into places of its own: no barrier, no register and no line
 // of L1 holds them meanwhile (through registers an SM had half as many bytes under way).
+// Two CTAs to an SM up to rank 64 (F32: up to 32), one beyond: shared memory, 124 KB for F32 at rank 64.
 template <typename W, uint32_t RP>
 __global__ void __launch_bounds__(THREADS, RP <= 64 ? 2 : 1) adapter_shrink_kernel(const __grid_constant__ ShrinkArgs<W> a) {
     namespace cg = cooperative_groups;
@@ -1163,9 +1164,11 @@ extern "C" size_t qw4sh_adapter_tiles(size_t tokens, uint32_t slots) {
 extern "C" int qw4sh_adapter_forward(const QW4ShTune *tune, const QW4CuAdapters *ad, const float *x, size_t x_pitch, const uint32_t *slots,
                                      const float *base, size_t base_pitch, float *y, size_t y_pitch, size_t tokens, void *stream) {
     const Rows xr = {x, x_pitch}, br = {base, base_pitch};
-    // A cluster per token costs a token its adapter out of L2 every time, the grouped products three launches: us, cluster | grouped, 2048 -> 2048
-    // unless said: rank 16 (2048 -> 512) 128 tokens 8.6 | 15; rank 32 128 tokens 11 | 16; rank 64 64 tokens 11 | 19, 96 tokens 18 | 19, 128 tokens
-    // 21 | 19; rank 128 (512 -> 2048) 64 tokens 19 | 21, 96 tokens 30 | 21.
+    // A cluster per token costs a token its adapter out of L2 every time, the grouped products three launches and a tile of 128 rows for every adapter
+    // in use.  us, cluster | grouped, BF16, 2048 -> 2048, tokens spread evenly over 8 slots: rank 16 128 tokens 10.2 | 15.7, 192 tokens 14.8 | 16.1;
+    // rank 32 128 tokens 12.4 | 16.2, 192 tokens 17.7 | 16.8; rank 64 64 tokens 12.4 | 17.1, 80 tokens 17.4 | 17.2, 96 tokens 19.7 | 17.1; rank 128 64 tokens
+    // 20.5 | 26.2, 80 tokens 28.4 | 26.3.  With one slot, and 2048 -> 512 and 512 -> 2048, the rule's choice is at most 27% behind the other.
+    // It takes adapters to be shared: the more of them are in use the later the crossing comes (rank 64, 192 tokens: 31 | 28 with 24, 31 | 49 with 48 in use).
     if (tokens <= 64 || (tokens <= 192 && tokens * ad->rank <= 5120))
         return (ad->type == 0 ? few<float> : ad->type == 1 ? few<__half> : few<__nv_bfloat16>)(tune, ad, xr, slots, br, y, y_pitch, tokens, (cudaStream_t)stream);
     Shape s;
