@@ -20,13 +20,13 @@ namespace {
 constexpr uint32_t THREADS = 256;
 
 // Probability sums meet as 64-bit integers, whose sum has no order: multiples of 2^-40 in the first, and what is left of a share in multiples of
-// 2^-82 in the second, so that an unlikely expert's sum keeps FP32's bits too.  A share of 2^-16 and more has nothing left.  Neither
-// overflows: shares add up to no more than 2^20 tokens, and there are no more than that many of less than 2^42 each in the second.
-constexpr float UNIT = 1099511627776.0f, REST = 4835703278458516698824704.0f;        // 2^40, 2^82
-__device__ __forceinline__ void add_share(unsigned long long *sum, uint32_t to_rest, float v) {
-    const long long whole = __float2ll_rz(v * UNIT), rest = __float2ll_rn(fmaf((float)whole, -1.0f / UNIT, v) * REST);        // both exact but for the last rounding
-    if (whole) atomicAdd(sum, (unsigned long long)whole);
-    if (rest) atomicAdd(sum + to_rest, (unsigned long long)rest);
+// 2^-82 in the second, so that an unlikely expert's sum keeps FP32's bits too.  Neither overflows: shares add up to no more than 2^20 tokens, and there
+// are no more than that many of less than 2^42 each in the second.
+constexpr uint32_t WHOLE = 40, REST = 82;
+__host__ __device__ constexpr float two_to(uint32_t n) { return (float)(1ull << n / 2) * (float)(1ull << (n - n / 2)); }
+// What v leaves of its multiples of 1 / unit (a power of two; nothing of a v of 2^24 of them or more), in multiples of 2^-REST.
+__device__ __forceinline__ unsigned long long rest_of(float v, float unit) {
+    return (unsigned long long)__float2ll_rn(fmaf(v, unit, -(float)__float2ll_rz(v * unit)) * (two_to(REST) / unit));
 }
 
 // By all lanes of a warp together: volatile, or the compiler may move it to where its result is used, which not every lane reaches.
@@ -88,6 +88,10 @@ template <int PER, bool VEC> struct Row {
     }
 };
 
+__device__ __forceinline__ void add_rest(const QW4ShTune &tune, uint32_t e, unsigned long long rest) {
+    if (rest) { atomicAdd(&tune.prob_rests[e], rest); tune.status[3] = 1; }
+}
+
 // The end of the forward pass: the CTA that arrives last hands the sums out and leaves zeros for the next launch.
 __device__ __forceinline__ void balance_finish(uint32_t E, const QW4ShTune &tune, uint32_t *counts, float *prob_sums, float *loss) {
     __shared__ uint32_t last;
@@ -100,15 +104,16 @@ __device__ __forceinline__ void balance_finish(uint32_t E, const QW4ShTune &tune
     if (!last) return;
     __threadfence();
     const uint32_t n = __ldcg(&tune.counts[E]);
-    const bool bad = __ldcg(tune.status + 2);
+    const bool bad = __ldcg(tune.status + 2), rests = __ldcg(tune.status + 3);
     double l = 0;
     for (uint32_t e = threadIdx.x; e < E; e += THREADS) {
         const uint32_t c = __ldcg(&tune.counts[e]);
-        const double p = (double)__ldcg(&tune.prob_sums[e]) * (1.0 / (double)UNIT) + (double)__ldcg(&tune.prob_sums[E + e]) * (1.0 / (double)REST);
+        double p = (double)__ldcg(&tune.prob_sums[e]) * (1.0 / (double)two_to(WHOLE));
+        if (rests) { p += (double)__ldcg(&tune.prob_rests[e]) * (1.0 / (double)two_to(REST)); tune.prob_rests[e] = 0; }
         counts[e] = c;
         prob_sums[e] = bad ? CUDART_NAN_F : (float)p;
         l += (double)c * p;
-        tune.counts[e] = 0; tune.prob_sums[e] = tune.prob_sums[E + e] = 0;
+        tune.counts[e] = 0; tune.prob_sums[e] = 0;
     }
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     if (lane == 0) part[warp] = l;
@@ -118,7 +123,7 @@ __device__ __forceinline__ void balance_finish(uint32_t E, const QW4ShTune &tune
         for (uint32_t w = 0; w < THREADS / 32; w++) l += part[w];
         *loss = bad ? CUDART_NAN_F : n ? (float)(l * (double)E / ((double)n * (double)n)) : 0.0f;
         counts[E] = n;
-        tune.counts[E] = 0; tune.counts[E + 1] = 0; tune.status[2] = 0;
+        tune.counts[E] = 0; tune.counts[E + 1] = 0; tune.status[2] = tune.status[3] = 0;
     }
 }
 
@@ -175,7 +180,11 @@ __global__ void __launch_bounds__(THREADS) balance_forward_kernel(uint32_t E, ui
         float sum = 0;
 #pragma unroll
         for (uint32_t w = 0; w < WARPS; w++) sum += sums[w * COLS + e];
-        add_share(&tune.prob_sums[e], E, sum);
+        const unsigned long long whole = (unsigned long long)__float2ll_rz(sum * two_to(WHOLE));
+        if (whole) atomicAdd(&tune.prob_sums[e], whole);
+        if (sum < two_to(24) / two_to(WHOLE)) {
+            add_rest(tune, e, rest_of(sum, two_to(WHOLE)));
+        }
         if (hist[e]) atomicAdd(&tune.counts[e], hist[e]);
     }
     if (threadIdx.x == 0 && rows_seen) atomicAdd(&tune.counts[E], rows_seen);
@@ -183,17 +192,19 @@ __global__ void __launch_bounds__(THREADS) balance_forward_kernel(uint32_t E, ui
 }
 
 // More experts than fit a warp's registers: a warp to a row, three passes over it (the later ones out of L1), every probability
-// added to the CTA's sums as an integer.
+// added to the CTA's sums as an integer, in multiples of 2^-unit: as fine as the CTA's rows leave room for.  What that leaves of a probability goes past
+// them, so that it takes no shared memory (two sums to an expert there: 8192 x 4096 157 us instead of 132).
 __global__ void __launch_bounds__(THREADS) balance_forward_wide_kernel(uint32_t E, uint32_t K, const float *logits, uint64_t pitch,
                                                                        const uint32_t *ids, const uint8_t *mask, uint32_t T,
-                                                                       const __grid_constant__ QW4ShTune tune, uint32_t *__restrict__ counts,
+                                                                       const __grid_constant__ QW4ShTune tune, uint32_t unit, uint32_t *__restrict__ counts,
                                                                        float *__restrict__ prob_sums, float *__restrict__ loss) {
-    extern __shared__ uint32_t shared_words[];               // [E] counts, [2][E] sums as 64-bit integers
+    extern __shared__ uint32_t shared_words[];               // [E] counts, [E] sums as 64-bit integers
     uint32_t *hist = shared_words;
     unsigned long long *sums = (unsigned long long *)(hist + ((E + 1) & ~1u));
     __shared__ uint32_t rows_seen;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (uint32_t e = threadIdx.x; e < E; e += THREADS) { hist[e] = 0; sums[e] = sums[E + e] = 0; }
+    const float scale = two_to(unit), few_bits = two_to(24) / scale;
+    for (uint32_t e = threadIdx.x; e < E; e += THREADS) { hist[e] = 0; sums[e] = 0; }
     if (threadIdx.x == 0) rows_seen = 0;
     grid_wait();
     __syncthreads();
@@ -207,7 +218,17 @@ __global__ void __launch_bounds__(THREADS) balance_forward_wide_kernel(uint32_t 
         s = warp_sum(s);
         if (!(s < CUDART_INF_F)) { if (lane == 0) { note_nonfinite(tune.status, t); tune.status[2] = 1; } }
         const float inv = 1.0f / s;
-        for (uint32_t e = lane; e < E; e += 32) add_share(&sums[e], E, expf(z[e] - m) * inv);
+        bool small = false;
+        for (uint32_t e = lane; e < E; e += 32) {
+            const float p = expf(z[e] - m) * inv;
+            small |= p < few_bits && p > 0;
+            atomicAdd(&sums[e], (unsigned long long)__float2ll_rz(p * scale));
+        }
+        if (small)                                           // a pass of its own: inside the other one it cost that a tenth
+            for (uint32_t e = lane; e < E; e += 32) {
+                const float p = expf(z[e] - m) * inv;
+                if (p < few_bits) add_rest(tune, e, rest_of(p, scale));
+            }
         for (uint32_t k = lane; k < K; k += 32) {
             const uint32_t e = ids[(uint64_t)t * K + k];
             if (e < E) atomicAdd(&hist[e], 1u); else atomicOr(tune.status, QW4SH_ERR_BOUNDS);
@@ -217,8 +238,9 @@ __global__ void __launch_bounds__(THREADS) balance_forward_wide_kernel(uint32_t 
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < E; e += THREADS) {
         if (hist[e]) atomicAdd(&tune.counts[e], hist[e]);
-        if (sums[e]) atomicAdd(&tune.prob_sums[e], sums[e]);
-        if (sums[E + e]) atomicAdd(&tune.prob_sums[E + e], sums[E + e]);
+        const unsigned long long whole = sums[e] >> (unit - WHOLE), rest = sums[e] - (whole << (unit - WHOLE)) << (REST - unit);
+        if (whole) atomicAdd(&tune.prob_sums[e], whole);
+        add_rest(tune, e, rest);
     }
     if (threadIdx.x == 0 && rows_seen) atomicAdd(&tune.counts[E], rows_seen);
     balance_finish(E, tune, counts, prob_sums, loss);
@@ -403,8 +425,12 @@ extern "C" int qw4sh_balance_forward(const QW4ShTune *tune, uint32_t E, uint32_t
                                 (uint32_t)tokens, *tune, counts, prob_sums, loss)
     if (E <= 1024) return BY_ROW(balance_forward_kernel, RUN);
 #undef RUN
-    return launch(balance_forward_wide_kernel, "balance_forward_wide_kernel", grid_of(tokens, 4), (size_t)((E + 1) & ~1u) * 4 + (size_t)E * 16, stream, E, K, logits,
-                  pitch, ids, mask, (uint32_t)tokens, *tune, counts, prob_sums, loss);
+    const unsigned grid = grid_of(tokens, 4);
+    const size_t rows = (tokens + grid * (THREADS / 32) - 1) / (grid * (THREADS / 32)) * (THREADS / 32);                       // of a CTA
+    uint32_t unit = 62;
+    while (rows > 1ull << (62 - unit)) unit--;
+    return launch(balance_forward_wide_kernel, "balance_forward_wide_kernel", grid, (size_t)((E + 1) & ~1u) * 4 + (size_t)E * 8, stream, E, K, logits,
+                  pitch, ids, mask, (uint32_t)tokens, *tune, unit, counts, prob_sums, loss);
 }
 
 extern "C" int qw4sh_balance_backward(const QW4ShTune *tune, uint32_t E, uint32_t K, int norm, const float *logits, size_t pitch, const uint32_t *ids,

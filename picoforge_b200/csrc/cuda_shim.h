@@ -249,9 +249,9 @@ int qw4sh_observed_forward(const QW4ShLayer *layer, const QW4ShWork *work, const
 int qw4sh_route_forward(const QW4ShLayer *layer, const QW4ShWork *work, const float *x, size_t tokens, int router_mode);
 /* Adapters and balance loss (adapters.cu, balance.cu): device scratch of one QW4CuTuneWork. */
 struct QW4ShTune {
-    uint32_t *status;             /* [4]: error bits, lowest bad row, whether this forward pass of the loss met one */
+    uint32_t *status;             /* [4]: error bits, lowest bad row; whether this forward pass of the loss met one, and has rests */
     /* balance loss: sums over the CTAs of a launch, zero between launches */
-    unsigned long long *prob_sums;    /* [2][experts of the call]: units of 2^-40, then of 2^-82 */
+    unsigned long long *prob_sums, *prob_rests;       /* [experts] units of 2^-40 and of 2^-82 */
     uint32_t *counts;             /* [experts + 1], and one ticket behind them */
     /* adapters: tokens sorted by slot, and tiles of them (16 bytes each) */
     uint32_t *order, *offsets;    /* [qw4sh_adapter_rows(tokens, slots)], [slots + 1][start, tokens] */

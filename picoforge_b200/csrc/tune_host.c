@@ -59,7 +59,8 @@ Qwen4Status qw4cu_tune_work_create(const QW4CuTuneLimits *limits, QW4CuTuneWork 
     w->limits = l;
     w->device = qw4sh_current_device();
     size_t at = 0;
-    const size_t status = take(&at, 16), sums = take(&at, (size_t)l.experts * 16), counts = take(&at, ((size_t)l.experts + 2) * 4);
+    const size_t status = take(&at, 16), sums = take(&at, (size_t)l.experts * 8), counts = take(&at, ((size_t)l.experts + 2) * 4);
+    const size_t rests = take(&at, (size_t)l.experts * 8);
     w->clear_bytes = at;
     const bool adapters = l.slots != 0;
     const size_t places = adapters ? qw4sh_adapter_rows(l.tokens, l.slots) : 0;
@@ -78,6 +79,7 @@ Qwen4Status qw4cu_tune_work_create(const QW4CuTuneLimits *limits, QW4CuTuneWork 
     }
     w->d.status = (uint32_t *)(w->block + status);
     w->d.prob_sums = (unsigned long long *)(w->block + sums);
+    w->d.prob_rests = (unsigned long long *)(w->block + rests);
     w->d.counts = (uint32_t *)(w->block + counts);
     w->d.order = (uint32_t *)(w->block + order);
     w->d.offsets = (uint32_t *)(w->block + offsets);
