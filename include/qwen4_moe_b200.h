@@ -585,7 +585,8 @@ typedef struct {
 /* y[t] = base[t] + scale_s B_s (A_s x[t]) with s = slots_dev[t]; y[t] = base[t] where that is QW4CU_NO_ADAPTER (or
  * out of range).  base NULL: zero; base may be y itself (same pitch), otherwise y must not overlap what is read.
  * Pitches are bytes between rows.  x [tokens, k], base and y [tokens, n].  Tokens of a slot may lie anywhere in the
- * batch.  Values enter the products with all their bits and are summed in FP32 (of products of two FP32 values 2^-21 at most is left out).
+ * batch.  base is the caller's: the layer's own products hand out nothing but y and the logits.  Values enter the
+ * products with all their bits and are summed in FP32 (of products of two FP32 values 2^-21 at most is left out).
  * An infinity or a NaN in an operand, and a sum beyond FP32's range, make those results not finite that the formula takes them to, and no others;
  * which of an infinity and a NaN comes out is not said and may depend on the number of tokens.  The same holds for the gradients. */
 Qwen4Status qw4cu_adapter_forward_device(const QW4CuAdapters *adapters, const float *x_dev, size_t x_pitch, const uint32_t *slots_dev,
@@ -602,8 +603,8 @@ Qwen4Status qw4cu_adapter_backward_device(const QW4CuAdapters *adapters, const f
 /* The layer's own router with the requests' adapters (k = hidden size, n = experts) beside it: logits of the router, scale B (A x) of every
  * token's slot on top, then the routes and, in the second call, the whole layer on them.  adapters NULL: the plain router (slots_dev and tune are
  * then not looked at).  logits_dev [tokens, experts], ids_dev and weights_dev [tokens, top_k] may be NULL; logits_dev receives what was
- * routed, which is what the balance loss wants, and must lie apart from every other argument.  Otherwise as qw4cu_moe_route_device and qw4cu_moe_forward_device, for up to 2048 tokens, without
- * the one-kernel decode path and without replay; bad slots are reported by qw4cu_tune_work_sync, everything else by qw4cu_moe_work_sync. */
+ * routed, which is what the balance loss wants, and must lie apart from every other argument.  Otherwise as
+ * qw4cu_moe_route_device and qw4cu_moe_forward_device, for up to 2048 tokens, without the one-kernel decode path and without replay; bad slots are reported by qw4cu_tune_work_sync, everything else by qw4cu_moe_work_sync. */
 Qwen4Status qw4cu_moe_route_adapted_device(const Qwen4Moe *moe, const float *x_dev, size_t tokens, const QW4CuAdapters *adapters,
                                            const uint32_t *slots_dev, QW4CuTuneWork *tune, float *logits_dev, uint32_t *ids_dev,
                                            float *weights_dev, Qwen4MoeWork *work, Qwen4Error *err);
@@ -627,7 +628,8 @@ Qwen4Status qw4cu_balance_forward_device(const Qwen4MoeConfig *config, const flo
                                          QW4CuTuneWork *work, Qwen4Error *err);
 /* Gradient of the router's logits: of loss_grad * loss, with the counts as they are (they may have been summed over
  * ranks, N included, for a loss over the whole batch of a job), plus, where weights_grad_dev [tokens, top_k] is given, that of the
- * route weights (normalised over the chosen experts if config->norm_topk_prob, plain probabilities otherwise) for it.
+ * route weights (normalised over the chosen experts if config->norm_topk_prob, plain probabilities otherwise) for it
+ * (the caller's: no call here works it out).
  * grad [tokens, experts] is overwritten; rows that the mask leaves out are zero. */
 Qwen4Status qw4cu_balance_backward_device(const Qwen4MoeConfig *config, const float *logits_dev, size_t logits_pitch, const uint32_t *ids_dev,
                                           const uint8_t *mask_dev, size_t tokens, const uint32_t *counts_dev, float loss_grad,
